@@ -353,6 +353,136 @@ int twg_abs(void *out, const void *a, int32_t dtype, const twg_iter_t *it, twg_s
 int twg_and(void *out, const void *a, const void *b, int32_t elem_size, const twg_iter_t *it,
             twg_stream_t stream);
 
+/* ---------------------------------------------- steps of a transformer layer
+ *
+ * Memory-bound steps that stand between a layer's matrix products.  They have no
+ * counterpart in the reference, whose registrations end at the activations and the CPU
+ * fallbacks (csrc/ops/activation_functions.cpp:116-126, csrc/bindings.cpp:32-43).
+ * Conventions as above, and:
+ *  - Element types are TWG_DT_F16, TWG_DT_BF16 and TWG_DT_F32; arithmetic is binary32
+ *    throughout and a result is rounded once, when it is stored.
+ *  - The calls allocate nothing, never wait and keep nothing between calls, so they may be
+ *    captured into a graph; where a call needs scratch, the caller brings it, and two calls
+ *    that may run at the same time need two.
+ *  - TWG_STREAM_NULL names the process's default (null) stream, which an opaque NULL
+ *    cannot (NULL is the library's own stream). */
+#define TWG_STREAM_NULL ((twg_stream_t)1)
+
+#define TWG_ROPE_MAX_HEAD_DIM 512
+#define TWG_ROPE_MAX_AXES 8
+
+/* The heads of one tensor, queries or keys: [batch, tokens, heads, head_dim] with unit
+ * stride along head_dim and any strides (in elements) along the other three, so that
+ * views of a packed projection and [batch, heads, tokens, head_dim] storage go in as they
+ * are.  Inputs may be broadcast (stride 0); outputs must not overlap anything but, in
+ * twg_norm_rope, their own input with the same strides (in place). */
+typedef struct twg_rope_part {
+  int64_t heads;        /* 0: this part is absent */
+  const void *x;        /* the heads before norm and rotation */
+  const void *dy;       /* backward: gradient of the rotated heads */
+  void *out;            /* forward: rotated heads; backward: gradient of x */
+  const void *weight;   /* norm weight [head_dim] of weight_dtype; NULL = ones */
+  void *dweight;        /* backward: gradient of the weight, of weight_dtype, or NULL */
+  int64_t x_stride[3];  /* batch, token, head */
+  int64_t dy_stride[3];
+  int64_t out_stride[3];
+} twg_rope_part_t;
+
+typedef struct twg_norm_rope {
+  int32_t dtype;          /* of x, dy and out */
+  int32_t weight_dtype;   /* of weight and dweight */
+  int32_t position_dtype; /* TWG_DT_I32, TWG_DT_I64 or TWG_DT_F32 */
+  int32_t norm;           /* 0: rotation only (weight, dweight and eps are not used) */
+  int32_t adjacent;       /* 0: pair i = elements (i, i + rot_dim/2); 1: (2i, 2i + 1) */
+  int32_t n_axes;         /* 1..TWG_ROPE_MAX_AXES */
+  int32_t head_dim;       /* even, 2..TWG_ROPE_MAX_HEAD_DIM */
+  int32_t rot_dim;        /* even, 0..head_dim: elements beyond it are not rotated */
+  float eps;
+  int32_t reserved;
+  int64_t batch;
+  int64_t tokens;
+  const void *positions;  /* [n_axes, batch, tokens] by pos_stride (any, 0 included) */
+  int64_t pos_stride[3];
+  const float *inv_freq;  /* [rot_dim / 2], device memory */
+  uint8_t pair_axis[TWG_ROPE_MAX_HEAD_DIM / 2]; /* position axis of each pair, < n_axes */
+  twg_rope_part_t part[2];
+} twg_norm_rope_t;
+
+/* RMS norm of every head and rotation of its pairs by position, queries and keys in one
+ * launch:  z = x * (mean(x^2) + eps)^(-1/2) * weight;  with a = position[pair_axis[i]] *
+ * inv_freq[i], pair (lo, hi) becomes (lo cos a - hi sin a, hi cos a + lo sin a).  Angles are
+ * formed and reduced in binary64, so positions of many millions keep their fraction of a
+ * turn.  Several axes (time, height, width) are chosen pair by pair. */
+int twg_norm_rope(const twg_norm_rope_t *d, twg_stream_t stream);
+/* Gradients of the above: dx into part[].out, the weights' into part[].dweight (summed over
+ * batch, tokens and heads in a fixed order: equal calls give equal bits).  x are the
+ * inputs of the forward call; without the norm x is not read and may be NULL. */
+int twg_norm_rope_backward(const twg_norm_rope_t *d, void *scratch, size_t scratch_bytes,
+                           twg_stream_t stream);
+/* Bytes of device scratch the backward call needs (0 where no dweight is asked for). */
+size_t twg_norm_rope_backward_scratch_bytes(const twg_norm_rope_t *d);
+
+#define TWG_LOGPROBS_MAX_TOP_K 64
+
+/* Log probabilities of one given token per row of logits [rows, vocab] (unit stride along
+ * vocab, rows row_stride elements apart), with c = scale > 0 (one over the temperature),
+ * m = max x, s = sum exp(c (x - m)):
+ *   logprob = c (x[target] - m) - log s;  0 where the target is ignore_index;  NaN where it is
+ *             neither that nor in 0..vocab-1
+ *   entropy = log s - sum p c (x - m), nats
+ *   top_logprobs / top_ids [rows, top_k]: the largest entries in descending order, the lowest
+ *             id first among equals (NaN ranks above everything)
+ * -inf entries are masked: p = 0, no contribution.  A row with nothing else (s = 0) has
+ * logprob and top_logprobs -inf and entropy 0.  +inf or NaN in a row makes its results NaN. */
+typedef struct twg_token_logprobs {
+  int32_t dtype;        /* of logits and grad */
+  int32_t target_dtype; /* TWG_DT_I32 or TWG_DT_I64 */
+  int64_t rows;
+  int64_t vocab;        /* 1..2^31 - 1 */
+  int64_t row_stride;
+  const void *logits;
+  const void *targets;  /* [rows] */
+  int64_t ignore_index;
+  float scale;
+  int32_t top_k;        /* 0..min(vocab, TWG_LOGPROBS_MAX_TOP_K) */
+  float *logprob;       /* [rows] each; forward: NULL = not wanted */
+  float *entropy;
+  float *row_max;       /* m */
+  float *row_sum;       /* s */
+  float *top_logprobs;
+  int64_t *top_ids;
+  const float *g_logprob; /* backward: incoming gradients [rows], NULL = 0 */
+  const float *g_entropy;
+  void *grad;           /* backward: [rows, vocab], rows grad_stride apart; may be logits itself */
+  int64_t grad_stride;
+} twg_token_logprobs_t;
+
+int twg_token_logprobs(const twg_token_logprobs_t *d, void *scratch, size_t scratch_bytes,
+                       twg_stream_t stream);
+/* Bytes of device scratch the forward call needs (0 where every row is one workgroup's). */
+size_t twg_token_logprobs_scratch_bytes(const twg_token_logprobs_t *d);
+/* grad[j] = c (g_logprob ([j == target] - p[j]) - g_entropy p[j] (log p[j] + entropy)) from
+ * the forward call's row_max, row_sum and entropy (the last only where g_entropy is given).
+ * The top alternatives carry no gradient.  Ignored targets take no part in the first term;
+ * a row without entries (s = 0) and a row whose two incoming gradients are 0 get zeros
+ * (the latter whatever its logits hold: nothing of them is read). */
+int twg_token_logprobs_backward(const twg_token_logprobs_t *d, twg_stream_t stream);
+
+/* out = residual + keep * x * scale (residual NULL: without it), its own backward pass when
+ * called on the incoming gradient.  `it` as for twg_add_f32 (TWG_A = x, TWG_B = residual), but
+ * the order of the dimensions counts, as for masked_select: element e is the e-th with
+ * dimension 0 fastest.  Its 16 random bits are half h = e % 2 (0: lower) of word (e / 2) % 4 of
+ * Philox4x32-10 (Salmon, Moraes, Dror, Shaw: Parallel random numbers, SC 2011) with
+ * counter {e/8, e/8 >> 32, offset, offset >> 32} and key {seed, seed >> 32}; it is dropped
+ * where they are below T = floor(65536 p + 0.5), and scale = 65536 / (65536 - T): p is rounded
+ * to a multiple of 2^-16 and the expectation is exact for the rounded one.  A dropped element
+ * contributes 0 whatever x holds; T = 65536 drops all.  No mask is stored.
+ * d_offset (device memory, or NULL) is added to offset when the kernel runs, so that a
+ * captured graph can draw anew in each replay.  out may be x or residual itself. */
+int twg_dropout(void *out, const void *x, const void *residual, int32_t dtype, double p,
+                uint64_t seed, uint64_t offset, const uint64_t *d_offset, const twg_iter_t *it,
+                twg_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

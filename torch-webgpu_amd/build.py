@@ -2,7 +2,7 @@
 """In-tree build of the two native pieces of torch_webgpu (MI355X / gfx950).
 
   libtwg_hip.so   torch-free HIP kernel library behind the C ABI of include/twg.h
-                  (hipcc --offload-arch=gfx950 over csrc/hip/*.hip)
+                  (hipcc --offload-arch=gfx950 over csrc/hip/*.hip and csrc/nn/*.hip)
   _C.so           the torch-facing extension: allocator, device guard and the
                   TORCH_LIBRARY_IMPL(aten, PrivateUse1) registrations
                   (g++ over csrc/torch/*.cpp, linked against libtwg_hip.so)
@@ -43,6 +43,7 @@ HIP_FLAGS = [
     "-Wno-unused-function",
     "-I" + INCLUDE,
     "-I" + os.path.join(HERE, "csrc", "hip"),
+    "-I" + os.path.join(HERE, "csrc", "nn"),
 ]
 
 
@@ -67,6 +68,7 @@ def build_hip(nproc=8, extra_flags=()):
     hipcc = shutil.which("hipcc") or os.path.join(ROCM, "bin", "hipcc")
     os.makedirs(OBJ, exist_ok=True)
     srcs = sorted(glob.glob(os.path.join(HERE, "csrc", "hip", "*.hip")))
+    srcs += sorted(glob.glob(os.path.join(HERE, "csrc", "nn", "*.hip")))
     objs, jobs = [], []
     for s in srcs:
         o = os.path.join(OBJ, os.path.basename(s) + ".o")

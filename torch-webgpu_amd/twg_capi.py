@@ -6,6 +6,7 @@ of torch_webgpu._C so the kernels can be driven, tested and timed without the
 dispatcher in the way.  There is no CPU fallback: if the library is missing or a
 call fails, an exception is raised.
 """
+import collections
 import ctypes
 import os
 
@@ -52,6 +53,37 @@ class MemStats(ctypes.Structure):
                  "bytes_pending")]
 
 
+ROPE_MAX_HEAD_DIM, ROPE_MAX_AXES = 512, 8
+LOGPROBS_MAX_TOP_K = 64
+STREAM_NULL = 1  # TWG_STREAM_NULL: the process's null stream, for the calls on tensors below
+
+
+class RopePart(ctypes.Structure):
+    """twg_rope_part_t: the heads of one tensor, queries or keys."""
+    _fields_ = [("heads", ctypes.c_int64)] + [
+        (n, ctypes.c_void_p) for n in ("x", "dy", "out", "weight", "dweight")] + [
+        (n, ctypes.c_int64 * 3) for n in ("x_stride", "dy_stride", "out_stride")]
+
+
+class NormRope(ctypes.Structure):
+    """twg_norm_rope_t"""
+    _fields_ = [(n, ctypes.c_int32) for n in ("dtype", "weight_dtype", "position_dtype", "norm", "adjacent", "n_axes",
+                                              "head_dim", "rot_dim")] + [
+        ("eps", ctypes.c_float), ("reserved", ctypes.c_int32), ("batch", ctypes.c_int64), ("tokens", ctypes.c_int64),
+        ("positions", ctypes.c_void_p), ("pos_stride", ctypes.c_int64 * 3), ("inv_freq", ctypes.c_void_p),
+        ("pair_axis", ctypes.c_uint8 * (ROPE_MAX_HEAD_DIM // 2)), ("part", RopePart * 2)]
+
+
+class TokenLogprobsArgs(ctypes.Structure):
+    """twg_token_logprobs_t"""
+    _fields_ = [("dtype", ctypes.c_int32), ("target_dtype", ctypes.c_int32), ("rows", ctypes.c_int64),
+                ("vocab", ctypes.c_int64), ("row_stride", ctypes.c_int64), ("logits", ctypes.c_void_p),
+                ("targets", ctypes.c_void_p), ("ignore_index", ctypes.c_int64), ("scale", ctypes.c_float),
+                ("top_k", ctypes.c_int32)] + [
+        (n, ctypes.c_void_p) for n in ("logprob", "entropy", "row_max", "row_sum", "top_logprobs", "top_ids", "g_logprob",
+                                       "g_entropy", "grad")] + [("grad_stride", ctypes.c_int64)]
+
+
 # Every symbol include/twg.h declares; tests check that the library exports them all.
 SYMBOLS = [
     "twg_init", "twg_is_initialized", "twg_error_string", "twg_device_info",
@@ -66,6 +98,9 @@ SYMBOLS = [
     "twg_masked_select_scratch_bytes", "twg_masked_select_f32", "twg_masked_select_count",
     "twg_masked_select_f32_static", "twg_masked_select_f32_wait_probe",
     "twg_eq", "twg_ne_scalar", "twg_and", "twg_abs",
+    "twg_norm_rope", "twg_norm_rope_backward", "twg_norm_rope_backward_scratch_bytes",
+    "twg_token_logprobs", "twg_token_logprobs_scratch_bytes", "twg_token_logprobs_backward",
+    "twg_dropout",
 ]
 
 _lib = None
@@ -129,6 +164,16 @@ def load():
     L.twg_ne_scalar.argtypes = [vp, vp, i32, ctypes.c_double, i64, ip, vp]
     L.twg_and.argtypes = [vp, vp, vp, i32, ip, vp]
     L.twg_abs.argtypes = [vp, vp, i32, ip, vp]
+    rp, lp, u64 = ctypes.POINTER(NormRope), ctypes.POINTER(TokenLogprobsArgs), ctypes.c_uint64
+    L.twg_norm_rope.argtypes = [rp, vp]
+    L.twg_norm_rope_backward.argtypes = [rp, vp, sz, vp]
+    L.twg_norm_rope_backward_scratch_bytes.argtypes = [rp]
+    L.twg_norm_rope_backward_scratch_bytes.restype = sz
+    L.twg_token_logprobs.argtypes = [lp, vp, sz, vp]
+    L.twg_token_logprobs_scratch_bytes.argtypes = [lp]
+    L.twg_token_logprobs_scratch_bytes.restype = sz
+    L.twg_token_logprobs_backward.argtypes = [lp, vp]
+    L.twg_dropout.argtypes = [vp, vp, vp, i32, ctypes.c_double, u64, u64, vp, ip, vp]
     _lib = L
     return L
 
@@ -278,3 +323,236 @@ class Event:
             load().twg_event_destroy(self.ev)
         except Exception:
             pass
+
+
+# ------------------------------------------------- steps of a transformer layer, on tensors
+#
+# The same entry points called on torch tensors whose memory the GPU addresses: tensors of the
+# "webgpu" device (the work goes to the library's stream) or of PyTorch-ROCm's device 0 (it goes
+# to torch's current stream, so it is ordered with torch's own products there and can be
+# captured with them).  Results and scratch are allocated with torch on the same device.
+# Arguments are checked here; what the library refuses raises TwgError.
+
+_FLOATS = (torch.float16, torch.bfloat16, torch.float32)
+_POSITIONS = (torch.int32, torch.int64, torch.float32)
+
+
+def _require(ok, message):
+    if not ok:
+        raise ValueError(message)
+
+
+def _stream_for(t):
+    """The stream argument for work on t."""
+    if t.device.type == "cuda":
+        _require(t.device.index == 0, "the library is bound to device 0")
+        return torch.cuda.current_stream(t.device).cuda_stream or STREAM_NULL
+    _require(t.device.type == "webgpu", f"expected a tensor in GPU memory, got {t.device}")
+    return None
+
+
+def _same_device(first, *others):
+    for t in others:
+        _require(t is None or t.device == first.device, "all tensors must be on one device")
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+def _norm_rope_args(q, k, positions, inv_freq, q_weight, k_weight, eps, pair_axis, adjacent):
+    _require(q.dim() == 4 and q.dtype in _FLOATS, "q must be [batch, tokens, heads, head_dim] of float16, bfloat16 or float32")
+    B, T, _, D = q.shape
+    _require(k is None or (k.dim() == 4 and k.shape[:2] == q.shape[:2] and k.shape[3] == D and k.dtype == q.dtype),
+             "k must have q's dtype and shape up to the number of heads")
+    _require(positions.dim() in (1, 2, 3) and positions.dtype in _POSITIONS,
+             "positions must be [tokens], [batch, tokens] or [axes, batch, tokens] of int32, int64 or float32")
+    _same_device(q, k, positions, inv_freq, q_weight, k_weight)
+    _require(inv_freq.dim() == 1 and inv_freq.dtype == torch.float32 and inv_freq.is_contiguous(),
+             "inv_freq must be a contiguous float32 vector, one entry per rotated pair")
+    axes = positions.shape[0] if positions.dim() == 3 else 1
+    _require(tuple(positions.shape) == ((T,), (B, T), (axes, B, T))[positions.dim() - 1], "positions do not fit q")
+    _require(2 * inv_freq.shape[0] <= D <= ROPE_MAX_HEAD_DIM, "more pairs than the head has, or a head beyond 512 elements")
+    _require(1 <= axes <= ROPE_MAX_AXES, "1 to 8 position axes")
+    _require(pair_axis is None or len(pair_axis) == inv_freq.shape[0], "pair_axis must name an axis for each rotated pair")
+    _require(pair_axis is not None or axes == 1, "several position axes need pair_axis")
+    _require(eps is not None or (q_weight is None and k_weight is None), "weights without a norm (eps is None)")
+    d = NormRope()
+    d.dtype = d.weight_dtype = DTYPES[q.dtype]
+    for w in (q_weight, k_weight):
+        if w is not None:
+            _require(w.shape == (D,) and w.is_contiguous() and w.dtype in (q.dtype, torch.float32),
+                     "a norm weight must be a contiguous vector [head_dim] of q's dtype or float32")
+            d.weight_dtype = DTYPES[w.dtype]
+    _require(q_weight is None or k_weight is None or q_weight.dtype == k_weight.dtype, "norm weights of two dtypes")
+    d.position_dtype = DTYPES[positions.dtype]
+    d.norm, d.eps = (0, 0.0) if eps is None else (1, eps)
+    d.adjacent, d.n_axes, d.head_dim, d.rot_dim = int(adjacent), axes, D, 2 * inv_freq.shape[0]
+    d.batch, d.tokens = B, T
+    d.positions, d.inv_freq = positions.data_ptr(), inv_freq.data_ptr()
+    st = positions.stride()
+    d.pos_stride[:] = ((0, 0) + st, (0,) + st, st)[positions.dim() - 1]
+    if pair_axis is not None:
+        ctypes.memmove(d.pair_axis, bytes(pair_axis), len(pair_axis))
+    for i, (x, w) in enumerate(((q, q_weight), (k, k_weight))):
+        if x is not None:
+            p = d.part[i]
+            p.heads, p.weight = x.shape[2], _ptr(w)
+    return d
+
+
+def _dense_heads(x):
+    """x, or a copy of it, with unit stride along the last dimension."""
+    return x if x.stride(3) == 1 or x.shape[3] == 1 else x.contiguous()
+
+
+def norm_rope(q, k, positions, inv_freq, q_weight=None, k_weight=None, eps=1e-6, pair_axis=None, adjacent=False,
+              q_out=None, k_out=None):
+    """RMS norm of every head of q and k and rotation by position: (q_out, k_out).
+
+    q, k: [batch, tokens, heads, head_dim], any strides (views of a packed projection, heads
+    first); k may be None.  eps=None leaves the norm out.  positions: [tokens], [batch, tokens]
+    or [axes, batch, tokens]; inv_freq: one frequency per rotated pair (2 * len(inv_freq) elements of
+    a head are rotated, the rest passes through); pair_axis: for each pair the position axis it
+    follows (bytes or a list).  adjacent: pairs are neighbours (2i, 2i + 1) instead of halves.
+    q_out / k_out: where the results go (unit stride along head_dim); q and k themselves for a
+    call in place."""
+    stream = _stream_for(q)
+    d = _norm_rope_args(q, k, positions, inv_freq, q_weight, k_weight, eps, pair_axis, adjacent)
+    outs = []
+    for i, (x, out) in enumerate(((q, q_out), (k, k_out))):
+        if x is None:
+            _require(out is None, "an output without its input")
+            outs.append(None)
+            continue
+        if out is None:
+            out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        else:
+            _same_device(x, out)
+            _require(out.shape == x.shape and out.dtype == x.dtype and (out.stride(3) == 1 or out.shape[3] == 1),
+                     "an output must have its input's shape and dtype and unit stride along head_dim")
+        x = _dense_heads(x)
+        p = d.part[i]
+        p.x, p.out = x.data_ptr(), out.data_ptr()
+        p.x_stride[:], p.out_stride[:] = x.stride()[:3], out.stride()[:3]
+        outs.append(out)
+    check(load().twg_norm_rope(ctypes.byref(d), stream))
+    return tuple(outs)
+
+
+def norm_rope_backward(dq, dk, q, k, positions, inv_freq, q_weight=None, k_weight=None, eps=1e-6, pair_axis=None,
+                       adjacent=False):
+    """Gradients of norm_rope for the incoming gradients dq and dk of its results:
+    (grad q, grad k, grad q_weight, grad k_weight), None for what the call does not have."""
+    stream = _stream_for(q)
+    d = _norm_rope_args(q, k, positions, inv_freq, q_weight, k_weight, eps, pair_axis, adjacent)
+    grads, keep = [None] * 4, []
+    for i, (x, dy, w) in enumerate(((q, dq, q_weight), (k, dk, k_weight))):
+        if x is None:
+            _require(dy is None, "a gradient without its input")
+            continue
+        _same_device(x, dy)
+        _require(dy.shape == x.shape and dy.dtype == x.dtype, "an incoming gradient must have its input's shape and dtype")
+        x, dy = _dense_heads(x), _dense_heads(dy)
+        keep.append((x, dy))
+        grads[i] = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        p = d.part[i]
+        p.x, p.dy, p.out = x.data_ptr(), dy.data_ptr(), grads[i].data_ptr()
+        p.x_stride[:], p.dy_stride[:], p.out_stride[:] = x.stride()[:3], dy.stride()[:3], grads[i].stride()[:3]
+        if w is not None:
+            grads[2 + i] = torch.empty_like(w)
+            p.dweight = grads[2 + i].data_ptr()
+    L = load()
+    need = L.twg_norm_rope_backward_scratch_bytes(ctypes.byref(d))
+    scratch = torch.empty(need // 4, dtype=torch.float32, device=q.device) if need else None
+    check(L.twg_norm_rope_backward(ctypes.byref(d), _ptr(scratch), need, stream))
+    return tuple(grads)
+
+
+TokenLogprobs = collections.namedtuple("TokenLogprobs", "logprob entropy row_max row_sum top_logprobs top_ids")
+
+
+def _rows(logits):
+    return logits if logits.stride(1) == 1 or logits.shape[1] == 1 else logits.contiguous()
+
+
+def _logprob_args(logits, targets, scale, ignore_index):
+    _require(logits.dim() == 2 and logits.dtype in _FLOATS, "logits must be [rows, vocab] of float16, bfloat16 or float32")
+    _require(targets.shape == logits.shape[:1] and targets.dtype in (torch.int32, torch.int64) and targets.is_contiguous(),
+             "targets must be a contiguous int32 or int64 vector, one per row")
+    _same_device(logits, targets)
+    d = TokenLogprobsArgs()
+    d.dtype, d.target_dtype = DTYPES[logits.dtype], DTYPES[targets.dtype]
+    d.rows, d.vocab = logits.shape
+    d.row_stride, d.logits, d.targets = logits.stride(0), logits.data_ptr(), targets.data_ptr()
+    d.ignore_index, d.scale = ignore_index, scale
+    return d
+
+
+def token_logprobs(logits, targets, top_k=0, scale=1.0, ignore_index=-100):
+    """TokenLogprobs of logits [rows, vocab] and one given token per row: its log probability
+    (0 where the token is ignore_index), the row's entropy, the maximum and sum that the backward
+    call takes, and the top_k alternatives (ties: the lowest id first), all float32 but the
+    int64 ids.  scale multiplies the logits (one over the temperature); -inf logits are masked."""
+    stream = _stream_for(logits)
+    logits = _rows(logits)
+    d = _logprob_args(logits, targets, scale, ignore_index)
+    _require(0 <= top_k <= min(LOGPROBS_MAX_TOP_K, d.vocab), "top_k must be in 0..min(64, vocab)")
+    rows, dev = d.rows, logits.device
+    stats = torch.empty((4, rows), dtype=torch.float32, device=dev)
+    top = torch.empty((rows, top_k), dtype=torch.float32, device=dev)
+    ids = torch.empty((rows, top_k), dtype=torch.int64, device=dev)
+    base = stats.data_ptr()
+    d.logprob, d.entropy, d.row_max, d.row_sum = (base + 4 * rows * i for i in range(4))
+    d.top_k, d.top_logprobs, d.top_ids = top_k, top.data_ptr(), ids.data_ptr()
+    L = load()
+    need = L.twg_token_logprobs_scratch_bytes(ctypes.byref(d))
+    scratch = torch.empty(need // 8, dtype=torch.int64, device=dev) if need else None
+    check(L.twg_token_logprobs(ctypes.byref(d), _ptr(scratch), need, stream))
+    return TokenLogprobs(stats[0], stats[1], stats[2], stats[3], top, ids)
+
+
+def token_logprobs_backward(g_logprob, g_entropy, logits, targets, row_max, row_sum, entropy=None, scale=1.0,
+                            ignore_index=-100, out=None):
+    """Gradient of the logits for the incoming gradients of logprob and entropy (either may be
+    None).  row_max, row_sum and entropy come from token_logprobs with the same scale.  out may
+    be logits itself."""
+    stream = _stream_for(logits)
+    src = _rows(logits)
+    d = _logprob_args(src, targets, scale, ignore_index)
+    for v in (g_logprob, g_entropy, row_max, row_sum, entropy):
+        _require(v is None or (v.shape == targets.shape and v.dtype == torch.float32 and v.is_contiguous()),
+                 "gradients and statistics must be contiguous float32 vectors, one entry per row")
+    _same_device(logits, g_logprob, g_entropy, row_max, row_sum, entropy, out)
+    if out is None:
+        out = torch.empty(src.shape, dtype=src.dtype, device=src.device)
+    else:
+        _require(out.shape == src.shape and out.dtype == src.dtype and (out.stride(1) == 1 or out.shape[1] == 1),
+                 "out must have the logits' shape and dtype and unit stride along vocab")
+    d.g_logprob, d.g_entropy = _ptr(g_logprob), _ptr(g_entropy)
+    d.row_max, d.row_sum, d.entropy = _ptr(row_max), _ptr(row_sum), _ptr(entropy)
+    d.grad, d.grad_stride = out.data_ptr(), out.stride(0)
+    check(load().twg_token_logprobs_backward(ctypes.byref(d), stream))
+    return out
+
+
+def dropout(x, p, seed, offset=0, residual=None, out=None, d_offset=None):
+    """residual + dropout(x), or dropout(x): elements are kept by Philox4x32-10 of (seed, offset,
+    element index), so the gradient of x is dropout(grad, p, seed, offset) and no mask exists.  Each call of a
+    training step takes an offset of its own.  p is rounded to a multiple of 2^-16.  d_offset: an
+    int64 tensor of one element, added to offset when the kernel runs (captured graphs)."""
+    stream = _stream_for(x)
+    _require(x.dtype in _FLOATS, "x must be float16, bfloat16 or float32")
+    _same_device(x, residual, out, d_offset)
+    if out is None:
+        out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    for t in (residual, out):
+        _require(t is None or (t.shape == x.shape and t.dtype == x.dtype), "x, residual and out must agree in shape and dtype")
+    _require(d_offset is None or (d_offset.dtype == torch.int64 and d_offset.numel() == 1), "d_offset must be one int64")
+    if x.is_contiguous() and out.is_contiguous() and (residual is None or residual.is_contiguous()):
+        it = dense_iter(x.numel())
+    else:
+        it = make_iter(x.shape, out.stride(), x.stride(), None if residual is None else residual.stride())
+    check(load().twg_dropout(out.data_ptr(), x.data_ptr(), _ptr(residual), DTYPES[x.dtype], p, seed & (2 ** 64 - 1),
+                             offset & (2 ** 64 - 1), _ptr(d_offset), ctypes.byref(it), stream))
+    return out
