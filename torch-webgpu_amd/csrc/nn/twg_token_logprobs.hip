@@ -4,6 +4,11 @@
 //   m = max x, s = sum e^(c (x - m)), logprob = c (x_t - m) - log s,
 //   entropy = log s - (1/s) sum e^(c (x - m)) c (x - m)
 //   grad_j = c (g_lp ([j = t] - p_j) - g_H p_j (log p_j + entropy)),  p_j = e^(c (x_j - m)) / s
+//
+// The forward pass reads the logits once: every lane keeps a running maximum and the two sums
+// relative to it, every wavefront a sorted list of its best alternatives, one per lane.  A row is
+// one workgroup's, or one wavefront's if it is short; few long rows are split over
+// several workgroups, whose results a second kernel joins.
 #include "twg_nn.h"
 
 namespace twg {
@@ -17,9 +22,11 @@ struct LogprobArgs {
   int64_t rows, row_stride, ignore_index;
   int32_t vocab, top_k;
   int32_t wide_targets;  // int64 instead of int32
+  int32_t splits;        // workgroups per row
   float scale;
   float *logprob, *entropy, *row_max, *row_sum, *top_logprobs;
   int64_t *top_ids;
+  uint64_t *scratch;  // with splits > 1: [rows][splits][top_k] keys, then [rows][splits] Run
   const float *g_logprob, *g_entropy;
   const float *in_max, *in_sum, *in_entropy;
   void *grad;
@@ -30,98 +37,129 @@ __device__ __forceinline__ int64_t target_of(const LogprobArgs &a, int64_t row) 
   return a.wide_targets ? ((const int64_t *)a.targets)[row] : (int64_t)((const int32_t *)a.targets)[row];
 }
 
-// Order of the alternatives as one number: the value (-0 as +0, NaN on top), then the lower id.
-__device__ __forceinline__ uint64_t key_of(float x, uint32_t id) {
+// Order of the alternatives as one number: the value (-0 as +0, NaN on top), then the lower
+// id.  0 is below every key.
+__device__ __forceinline__ uint32_t rank_of(float x) {
   const uint32_t b = __float_as_uint(x + 0.0f);
-  const uint32_t v = x != x ? 0xFFFFFFFFu : b ^ ((uint32_t)((int32_t)b >> 31) | 0x80000000u);
-  return (uint64_t)v << 32 | (uint32_t)~id;
+  return x != x ? 0xFFFFFFFFu : b ^ ((uint32_t)((int32_t)b >> 31) | 0x80000000u);
 }
-__device__ __forceinline__ float value_of(uint64_t key) {
-  const uint32_t v = (uint32_t)(key >> 32);
+__device__ __forceinline__ float value_of_rank(uint32_t v) {
   if (v == 0xFFFFFFFFu) return __uint_as_float(0x7FC00000u);
   return __uint_as_float(v & 0x80000000u ? v ^ 0x80000000u : ~v);
 }
+__device__ __forceinline__ uint64_t key_of(float x, uint32_t id) { return (uint64_t)rank_of(x) << 32 | (uint32_t)~id; }
+__device__ __forceinline__ float value_of(uint64_t key) { return value_of_rank((uint32_t)(key >> 32)); }
 __device__ __forceinline__ uint32_t id_of(uint64_t key) { return ~(uint32_t)key; }
 
-// A running softmax sum: m the largest entry so far, s = sum e^(c (x - m)) and
-// t = sum e^(c (x - m)) c (x - m), the last in base 2.  -inf entries add nothing; before the
-// first other entry m is -inf and s is 0.
+// A running softmax sum in base 2: with b = base(m), s = sum 2^(c2 x - b) and
+// t = sum 2^(c2 x - b) (c2 x - b), c2 = scale log2 e.  c2 x - b is one fused multiply-add, rounded
+// once.  base(m) is c2 m rounded to binary32; the rounding is the same in every term and
+// cancels.  It is kept within +-1e37, so that 2^(c2 x - b) stays finite arithmetic where the largest
+// entry so far is -inf or near the type's lowest value: such entries then add 0.
+// A row of nothing else, and one with infinities or NaN, is recognised by its
+// sum and done again by slow_row().
 struct Run {
   float m, s, t;
 };
 
-__device__ __forceinline__ float exponent(float x, float m, float c2) { return (x - m) * c2; }
-
-__device__ __forceinline__ void add_to(Run &r, float x, float c2) {
-  if (x > r.m) {
-    if (r.s > 0.0f) {
-      const float d = fmaxf(exponent(r.m, x, c2), -300.0f), f = exp2f(d);
-      r.t = f * __fmaf_rn(d, r.s, r.t);
-      r.s *= f;
-    }
-    r.m = x;
-  }
-  if (x == -INFINITY) return;
-  const float d = exponent(x, r.m, c2), e = exp2f(d);
-  r.s += e;
-  r.t = __fmaf_rn(e, fmaxf(d, -300.0f), r.t);
-}
+__device__ __forceinline__ float base_of(float m, float c2) { return fminf(fmaxf(m * c2, -1e37f), 1e37f); }
+__device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 
 __device__ __forceinline__ Run join(const Run &a, const Run &b, float c2) {
   const bool swap = b.m > a.m;
-  const Run &hi = swap ? b : a, &lo = swap ? a : b;
-  Run r = hi;
-  // (a sum that is 0 has no entries; one that is NaN is passed on)
-  if (lo.s != 0.0f) {
-    const float d = hi.m == lo.m ? 0.0f : fmaxf(exponent(lo.m, hi.m, c2), -300.0f), f = exp2f(d);
-    r.s += lo.s * f;
-    r.t += f * __fmaf_rn(d, lo.s, lo.t);
-  }
-  return r;
+  const float m = swap ? b.m : a.m;
+  const float hs = swap ? b.s : a.s, ht = swap ? b.t : a.t, ls = swap ? a.s : b.s, lt = swap ? a.t : b.t;
+  const float d = fmaxf(base_of(swap ? a.m : b.m, c2) - base_of(m, c2), -300.0f), f = exp2_fast(d);
+  return Run{m, __fmaf_rn(f, ls, hs), __fmaf_rn(f, __fmaf_rn(d, ls, lt), ht)};
 }
 
 __device__ __forceinline__ Run shuffled(const Run &r, int lanes) {
   return Run{__shfl_xor(r.m, lanes), __shfl_xor(r.s, lanes), __shfl_xor(r.t, lanes)};
 }
 
+// What a row's results are computed from: s against the true maximum, in base e.
+struct RowStats {
+  float m, s, log_s, entropy;
+};
+__device__ __forceinline__ RowStats stats_of(const Run &r, float c2) {
+  if (r.s == 0.0f) return RowStats{r.m, 0.0f, 0.0f, 0.0f};
+  const float shift = __fmaf_rn(r.m, c2, -base_of(r.m, c2)), l = log2f(r.s);
+  return RowStats{r.m, r.s * exp2_fast(-shift), kLn2f * (l - shift), kLn2f * (l - r.t / r.s)};
+}
+// Whether the sums say what they should: 1 or more (less the rounding of base(m)) and finite, or 0
+// in a row of -inf.
+__device__ __forceinline__ bool plain_row(const Run &r) {
+  return r.m == -INFINITY ? r.s == 0.0f : r.s >= 0.5f && r.s < INFINITY;
+}
 // (in base e: an entry of the type's lowest value times log2 e would leave binary32's range)
-__device__ __forceinline__ float log_prob(float x, const Run &r, float scale) {
-  return r.s == 0.0f ? -INFINITY : (x - r.m) * scale - kLn2f * log2f(r.s);
+__device__ __forceinline__ float log_prob(float x, const RowStats &r, float scale) {
+  return r.s == 0.0f ? -INFINITY : (x - r.m) * scale - r.log_s;
 }
 
-// one row by one workgroup
 template <typename T>
-__global__ void __launch_bounds__(kThreads) logprobs_rows(LogprobArgs a) {
-  __shared__ Run runs[kThreads / 64];
-  __shared__ uint64_t best[kThreads / 64];
-  const int64_t row = blockIdx.x;
-  const T *x = (const T *)a.logits + row * a.row_stride;
-  const float c2 = a.scale * kLog2e;
-  Run r{-INFINITY, 0.0f, 0.0f};
-  for (int i = threadIdx.x; i < a.vocab; i += kThreads) add_to(r, (float)x[i], c2);
-  for (int i = 1; i < 64; i <<= 1) r = join(r, shuffled(r, i), c2);
-  if ((threadIdx.x & 63) == 0) runs[threadIdx.x >> 6] = r;
-  __syncthreads();
-  r = runs[0];
-  for (int i = 1; i < kThreads / 64; ++i) r = join(r, runs[i], c2);
-  const bool empty = r.s == 0.0f;
-  const float log2_s = log2f(r.s);
-  if (threadIdx.x == 0) {
-    const int64_t t = target_of(a, row);
-    float lp = 0.0f;
-    if (t != a.ignore_index) {
-      lp = __uint_as_float(0x7FC00000u);
-      if (t >= 0 && t < a.vocab) lp = log_prob((float)x[t], r, a.scale);
-    }
-    if (a.logprob) a.logprob[row] = lp;
-    if (a.entropy) a.entropy[row] = empty ? 0.0f : kLn2f * (log2_s - r.t / r.s);
-    if (a.row_max) a.row_max[row] = r.m;
-    if (a.row_sum) a.row_sum[row] = r.s;
+__device__ __forceinline__ void put_row(const LogprobArgs &a, int64_t row, const RowStats &r) {
+  const int64_t t = target_of(a, row);
+  float lp = 0.0f;
+  if (t != a.ignore_index) {
+    lp = __uint_as_float(0x7FC00000u);
+    if (t >= 0 && t < a.vocab) lp = log_prob((float)((const T *)a.logits)[row * a.row_stride + t], r, a.scale);
   }
+  if (a.logprob) a.logprob[row] = lp;
+  if (a.entropy) a.entropy[row] = r.s == 0.0f ? 0.0f : r.entropy;
+  if (a.row_max) a.row_max[row] = r.m;
+  if (a.row_sum) a.row_sum[row] = r.s;
+}
+__device__ __forceinline__ void put_top(const LogprobArgs &a, int64_t row, int k, uint64_t key, const RowStats &r) {
+  if (a.top_ids) a.top_ids[row * a.top_k + k] = id_of(key);
+  if (a.top_logprobs) a.top_logprobs[row * a.top_k + k] = log_prob(value_of(key), r, a.scale);
+}
+
+// Any row, by its definition: one pass for the maximum, one for the sums, one for each alternative.
+// For rows that the single pass cannot do: nothing but entries near the type's limits,
+// infinities, NaN.  `room`: LDS for one value per wavefront, two of them.
+template <typename T, int WAVES>
+__device__ void slow_row(const LogprobArgs &a, int64_t row, uint64_t (*room)[WAVES]) {
+  const T *x = (const T *)a.logits + row * a.row_stride;
+  const int wave = threadIdx.x >> 6;
+  float *f0 = (float *)room[0], *f1 = (float *)room[1];
+  float m = -INFINITY;
+  for (int i = threadIdx.x; i < a.vocab; i += 64 * WAVES) m = fmaxf(m, (float)x[i]);
+  for (int i = 1; i < 64; i <<= 1) m = fmaxf(m, __shfl_xor(m, i));
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) f0[wave] = m;
+  __syncthreads();
+  for (int i = 0; i < WAVES; ++i) m = fmaxf(m, f0[i]);
+  float s = 0.0f, t = 0.0f;
+  for (int i = threadIdx.x; i < a.vocab; i += 64 * WAVES) {
+    const float v = (float)x[i];
+    if (v == -INFINITY) continue;
+    const float d = (v - m) * a.scale, e = expf(d);
+    s += e;
+    t = __fmaf_rn(e, fmaxf(d, -300.0f), t);
+  }
+  for (int i = 1; i < 64; i <<= 1) {
+    s += __shfl_xor(s, i);
+    t += __shfl_xor(t, i);
+  }
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) {
+    f0[wave] = s;
+    f1[wave] = t;
+  }
+  __syncthreads();
+  s = f0[0];
+  t = f1[0];
+  for (int i = 1; i < WAVES; ++i) {
+    s += f0[i];
+    t += f1[i];
+  }
+  const float log_s = logf(s);
+  const RowStats r{m, s, log_s, log_s - t / s};
+  if (threadIdx.x == 0) put_row<T>(a, row, r);
   uint64_t below = ~0ull;  // keys are unique: the next alternative is the largest key below the last
   for (int k = 0; k < a.top_k; ++k) {
     uint64_t mine = 0;
-    for (int i = threadIdx.x; i < a.vocab; i += kThreads) {
+    for (int i = threadIdx.x; i < a.vocab; i += 64 * WAVES) {
       const uint64_t key = key_of((float)x[i], (uint32_t)i);
       if (key < below && key > mine) mine = key;
     }
@@ -130,16 +168,269 @@ __global__ void __launch_bounds__(kThreads) logprobs_rows(LogprobArgs a) {
       mine = other > mine ? other : mine;
     }
     __syncthreads();
-    if ((threadIdx.x & 63) == 0) best[threadIdx.x >> 6] = mine;
+    if ((threadIdx.x & 63) == 0) room[0][wave] = mine;
     __syncthreads();
-    below = best[0];
-    for (int i = 1; i < kThreads / 64; ++i) below = best[i] > below ? best[i] : below;
-    if (threadIdx.x == 0) {
-      if (a.top_ids) a.top_ids[row * a.top_k + k] = id_of(below);
-      if (a.top_logprobs)
-        a.top_logprobs[row * a.top_k + k] = log_prob(value_of(below), r, a.scale);
+    below = room[0][0];
+    for (int i = 1; i < WAVES; ++i) below = room[0][i] > below ? room[0][i] : below;
+    if (threadIdx.x == 0) put_top(a, row, k, below, r);
+  }
+}
+
+// ---- a wavefront's best alternatives: lane l holds the l-th best key, 0 where there is none yet
+
+__device__ __forceinline__ uint64_t read_lane(uint64_t v, int lane) {
+  const uint32_t lo = __builtin_amdgcn_readlane((uint32_t)v, lane);
+  const uint32_t hi = __builtin_amdgcn_readlane((uint32_t)(v >> 32), lane);
+  return (uint64_t)hi << 32 | lo;
+}
+// the value of the lane below (DPP, a move across the whole wavefront)
+__device__ __forceinline__ uint64_t lane_below(uint64_t v) {
+  const uint32_t lo = __builtin_amdgcn_update_dpp(0u, (uint32_t)v, 0x138 /* wave_shr:1 */, 0xF, 0xF, false);
+  const uint32_t hi = __builtin_amdgcn_update_dpp(0u, (uint32_t)(v >> 32), 0x138, 0xF, 0xF, false);
+  return (uint64_t)hi << 32 | lo;
+}
+
+struct BestList {
+  uint64_t mine;  // this lane's entry
+  uint64_t kth;   // the last one that counts, the same in all lanes
+
+  // Put the keys of the lanes that have one better than the k-th into their places, one after
+  // the other: about 20 instructions each.
+  __device__ __forceinline__ void insert(uint64_t key, int k, int lane) {
+    uint64_t todo;
+    while ((todo = __ballot(key > kth)) != 0) {
+      const int from = __builtin_ctzll(todo);
+      const uint64_t in = read_lane(key, from);
+      const int place = __popcll(__ballot(mine > in));
+      const uint64_t below = lane_below(mine);
+      mine = lane < place ? mine : lane == place ? in : below;
+      kth = read_lane(mine, k - 1);
+      key = lane == from ? 0 : key;
     }
   }
+};
+
+// Of 64 lanes' values the k-th largest: every value's place by comparing it with all others.
+__device__ __forceinline__ uint32_t kth_of_lanes(uint32_t v, int k) {
+  int above = 0;
+#pragma unroll
+  for (int i = 0; i < 64; ++i) above += (uint32_t)__builtin_amdgcn_readlane(v, i) > v;
+  uint32_t least = above < k ? v : 0xFFFFFFFFu;
+  for (int i = 1; i < 64; i <<= 1) least = min(least, (uint32_t)__shfl_xor((int)least, i));
+  return least;
+}
+
+constexpr int kUnroll = 4;  // packs of 16 bytes a lane loads before it looks at the first
+
+// One row, or the part `split` of it, by one workgroup of WAVES wavefronts.
+template <typename T, int WAVES, bool TOP>
+__global__ void __launch_bounds__(64 * WAVES) logprobs_rows(LogprobArgs a) {
+  constexpr int E = 16 / (int)sizeof(T), N = E * kUnroll, THREADS = 64 * WAVES;
+  __shared__ Run runs[WAVES];
+  __shared__ uint64_t room[2][WAVES];
+  __shared__ uint32_t floors[WAVES];
+  __shared__ uint64_t lists[TOP ? WAVES * TWG_LOGPROBS_MAX_TOP_K : 1], joined[TOP ? TWG_LOGPROBS_MAX_TOP_K : 1];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, k = a.top_k;
+  const int64_t row = a.splits == 1 ? blockIdx.x : blockIdx.x / a.splits;
+  const int split = a.splits == 1 ? 0 : blockIdx.x - (int)row * a.splits;
+  const T *x = (const T *)a.logits + row * a.row_stride;
+  const float c2 = a.scale * kLog2e;
+
+  // elements before the first 16-byte boundary, whole packs, elements behind them
+  const int lead = (int)((-(uintptr_t)x & 15) / sizeof(T));
+  const int head = lead < a.vocab ? lead : a.vocab;
+  const int packs = (a.vocab - head) / E, tail = a.vocab - head - packs * E;
+  const int per = (packs + a.splits - 1) / a.splits;
+  const int first = min(split * per, packs), last = min(first + per, packs);
+  const Pack<T, E> *body = (const Pack<T, E> *)(x + head);
+
+  Run r{-INFINITY, 0.0f, 0.0f};
+  float b = base_of(r.m, c2);
+  BestList best{0, 0};
+  if (TOP && lane == 0) floors[wave] = 0;
+  if (TOP) __syncthreads();
+
+  // n values of this lane into its running sums
+  auto add = [&](const float *v, auto n) {
+    constexpr int COUNT = decltype(n)::value;
+    float top = v[0];
+#pragma unroll
+    for (int j = 1; j < COUNT; ++j) top = fmaxf(top, v[j]);
+    if (top > r.m) {
+      const float nb = base_of(top, c2), d = fmaxf(b - nb, -300.0f), f = exp2_fast(d);
+      r.t = f * __fmaf_rn(d, r.s, r.t);
+      r.s *= f;
+      r.m = top;
+      b = nb;
+    }
+#pragma unroll
+    for (int j = 0; j < COUNT; ++j) {
+      const float d = __fmaf_rn(v[j], c2, -b), e = exp2_fast(d);
+      r.s += e;
+      r.t = __fmaf_rn(e, fmaxf(d, -300.0f), r.t);
+    }
+    return top;
+  };
+  // the few single elements at an end of the row: the first lanes of the first wavefront
+  auto edge = [&](int from, int n) {
+    if (wave != 0 || n == 0) return;
+    const bool has = lane < n;
+    const float v = has ? (float)x[from + lane] : -INFINITY;
+    add(&v, std::integral_constant<int, 1>());
+    if (TOP) best.insert(has ? key_of(v, (uint32_t)(from + lane)) : 0, k, lane);
+  };
+
+  if (split == 0) edge(0, head);
+  for (int p = first; p < last; p += kUnroll * THREADS) {
+    Pack<T, E> raw[kUnroll];
+    bool in[kUnroll];
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) {
+      const int at = p + u * THREADS + (int)threadIdx.x;
+      in[u] = at < last;
+      raw[u] = load_pack<true>(body + (in[u] ? at : last - 1));
+    }
+    float v[N];
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u)
+#pragma unroll
+      for (int j = 0; j < E; ++j) v[u * E + j] = in[u] ? (float)raw[u].v[j] : -INFINITY;
+    const float top = add(v, std::integral_constant<int, N>());
+    if constexpr (TOP) {
+      // Which elements may be among the best.  An element of a later step has a higher id than
+      // everything in the list, so it has to be larger than the k-th.  At least k elements of the
+      // row are as large as the smallest of the wavefronts' `floors`, each the
+      // ceil(k / WAVES)-th best of its wavefront.  While the list is not full: at least k
+      // elements of this step are as large as the k-th largest of the lanes' maxima.
+      bool all = false;
+      uint32_t least;  // rank a candidate has to reach
+      if (best.kth == 0) {
+        least = kth_of_lanes(rank_of(top), k);
+        all = least == rank_of(-INFINITY);
+      } else {
+        least = (uint32_t)(best.kth >> 32) + 1;
+      }
+      if (WAVES > 1) {
+        uint32_t floor = 0xFFFFFFFFu;
+#pragma unroll
+        for (int w = 0; w < WAVES; ++w) floor = min(floor, __hip_atomic_load(&floors[w], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP));
+        least = max(least, floor);
+      }
+      if (all || __ballot(rank_of(top) >= least)) {
+        // above the value one rank below `least` (that of -0, which 0x7FFFFFFF would be, is not in use)
+        const float bar = value_of_rank(least - (least == 0x80000000u ? 2 : 1));
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+          const bool cand = all ? in[j / E] : v[j] > bar;
+          if (__ballot(cand)) {
+            const uint32_t id = (uint32_t)(head + (p + (j / E) * THREADS + (int)threadIdx.x) * E + j % E);
+            best.insert(cand ? key_of(v[j], id) : 0, k, lane);
+          }
+        }
+        if (WAVES > 1) {
+          const uint64_t at = read_lane(best.mine, (k + WAVES - 1) / WAVES - 1);
+          if (lane == 0) __hip_atomic_store(&floors[wave], (uint32_t)(at >> 32), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+        }
+      }
+    }
+  }
+  if (split == a.splits - 1) edge(a.vocab - tail, tail);
+
+  // join the lanes, then the wavefronts
+#pragma unroll
+  for (int i = 1; i < 64; i <<= 1) r = join(r, shuffled(r, i), c2);
+  if (WAVES > 1) {
+    if (lane == 0) runs[wave] = r;
+    if (TOP && lane < k) lists[wave * k + lane] = best.mine;
+    if (TOP && (int)threadIdx.x < k) joined[threadIdx.x] = 0;
+    __syncthreads();
+    r = runs[0];
+#pragma unroll
+    for (int i = 1; i < WAVES; ++i) r = join(r, runs[i], c2);
+    if (TOP) {  // the place of each key among all of them
+      if ((int)threadIdx.x < WAVES * k) {
+        const uint64_t key = lists[threadIdx.x];
+        int place = 0;
+        for (int i = 0; i < WAVES * k; ++i) place += lists[i] > key;
+        if (key && place < k) joined[place] = key;
+      }
+      __syncthreads();
+      best.mine = lane < k ? joined[lane] : 0;
+    }
+  }
+  if (a.splits > 1) {
+    const int64_t part = blockIdx.x;
+    if (TOP && (int)threadIdx.x < k) a.scratch[part * k + threadIdx.x] = best.mine;
+    if (threadIdx.x == 0) {
+      Run *to = (Run *)(a.scratch + a.rows * a.splits * k) + part;
+      *to = r;
+    }
+    return;
+  }
+  if (!plain_row(r)) {  // the same in all threads
+    slow_row<T, WAVES>(a, row, room);
+    return;
+  }
+  const RowStats st = stats_of(r, c2);
+  if (threadIdx.x == 0) put_row<T>(a, row, st);
+  if (TOP && (int)threadIdx.x < k) put_top(a, row, threadIdx.x, best.mine, st);
+}
+
+// the largest of the lanes' values, by moves within and across rows of 16 lanes (DPP)
+__device__ __forceinline__ uint32_t max_of_lanes(uint32_t v) {
+#define TWG_MAX_STEP(ctrl, rows) v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, ctrl, rows, 0xF, false))
+  TWG_MAX_STEP(0x111, 0xF);  // row_shr:1
+  TWG_MAX_STEP(0x112, 0xF);  // row_shr:2
+  TWG_MAX_STEP(0x114, 0xF);  // row_shr:4
+  TWG_MAX_STEP(0x118, 0xF);  // row_shr:8: lane 15 of each row has the row's
+  TWG_MAX_STEP(0x142, 0xA);  // row_bcast:15
+  TWG_MAX_STEP(0x143, 0xC);  // row_bcast:31: lane 63 has all
+#undef TWG_MAX_STEP
+  return (uint32_t)__builtin_amdgcn_readlane((int)v, 63);
+}
+
+constexpr int kMaxSplits = 64;  // one lane each when they are joined
+
+// The parts of a row, joined by one workgroup.
+template <typename T>
+__global__ void __launch_bounds__(kThreads) logprobs_join(LogprobArgs a) {
+  constexpr int WAVES = kThreads / 64;
+  __shared__ uint64_t lists[kMaxSplits * TWG_LOGPROBS_MAX_TOP_K];
+  __shared__ uint64_t room[2][WAVES];
+  __shared__ Run whole;
+  const int64_t row = blockIdx.x;
+  const int k = a.top_k, splits = a.splits;
+  for (int i = threadIdx.x; i < splits * k; i += kThreads) lists[i] = a.scratch[row * splits * k + i];
+  const float c2 = a.scale * kLog2e;
+  if (threadIdx.x < 64) {
+    const Run *parts = (const Run *)(a.scratch + a.rows * splits * k) + row * splits;
+    Run r{-INFINITY, 0.0f, 0.0f};
+    if ((int)threadIdx.x < splits) r = parts[threadIdx.x];
+#pragma unroll
+    for (int i = 1; i < 64; i <<= 1) r = join(r, shuffled(r, i), c2);
+    if (threadIdx.x == 0) whole = r;
+  }
+  __syncthreads();
+  if (!plain_row(whole)) {
+    slow_row<T, WAVES>(a, row, room);
+    return;
+  }
+  if (threadIdx.x >= 64) return;
+  const RowStats st = stats_of(whole, c2);
+  const int lane = threadIdx.x;
+  if (lane == 0) put_row<T>(a, row, st);
+  // Lane l stands at the next entry of part l's list.  The parts follow each other in the row, so
+  // of equal values the lowest lane's has the lowest id.
+  int at = 0;
+  uint64_t next = lane < splits && k ? lists[lane * k] : 0, mine = 0;
+  for (int i = 0; i < k; ++i) {
+    const uint32_t rank = (uint32_t)(next >> 32);
+    const int from = __builtin_ctzll(__ballot(rank == max_of_lanes(rank)));
+    const uint64_t key = read_lane(next, from);
+    if (lane == i) mine = key;
+    if (lane == from) next = ++at < k ? lists[lane * k + at] : 0;
+  }
+  if (lane < k) put_top(a, row, lane, mine, st);
 }
 
 template <typename T>
@@ -159,7 +450,7 @@ __global__ void __launch_bounds__(kThreads) logprobs_grad(LogprobArgs a) {
   for (int j = blockIdx.y * kThreads + threadIdx.x; j < a.vocab; j += gridDim.y * kThreads) {
     float g = 0.0f;
     if (!none) {
-      const float d = exponent((float)x[j], m, c2), p = exp2f(d) * inv_s;
+      const float d = ((float)x[j] - m) * c2, p = exp2_fast(d) * inv_s;
       const float logs = __fmaf_rn(fmaxf(d, -300.0f), kLn2f, shift);
       g = a.scale * ((j == t ? g_lp : 0.0f) - p * __fmaf_rn(g_h, logs, g_lp));
     }
@@ -208,6 +499,28 @@ LogprobArgs args_of(const twg_token_logprobs_t *d) {
   return a;
 }
 
+struct RowShape {
+  int waves;   // wavefronts per workgroup
+  int splits;  // workgroups per row
+};
+
+// A row that one wavefront reads in two steps is one wavefront's; few longer rows are split so that
+// there are about 1024 workgroups, each with one step of its own at least.
+RowShape shape_of(const twg_token_logprobs_t *d) {
+  const int64_t step = 16 * kUnroll / nn_size(d->dtype) * 64;  // elements a wavefront takes at a time
+  if (d->vocab <= 2 * step) return RowShape{1, 1};
+  int64_t splits = (1024 + d->rows - 1) / d->rows;
+  const int64_t steps = (d->vocab + 4 * step - 1) / (4 * step);
+  splits = splits < steps ? splits : steps;
+  return RowShape{4, (int)(splits < kMaxSplits ? splits : kMaxSplits)};
+}
+
+size_t scratch_of(const twg_token_logprobs_t *d, int splits) {
+  if (splits == 1) return 0;
+  const size_t parts = (size_t)d->rows * (size_t)splits;
+  return (parts * ((size_t)d->top_k * 8 + sizeof(Run)) + 7) / 8 * 8;
+}
+
 }  // namespace
 }  // namespace twg
 
@@ -215,21 +528,41 @@ using namespace twg;
 
 extern "C" {
 
-size_t twg_token_logprobs_scratch_bytes(const twg_token_logprobs_t *) { return 0; }
+size_t twg_token_logprobs_scratch_bytes(const twg_token_logprobs_t *d) {
+  return check(d, false) <= 0 ? 0 : scratch_of(d, shape_of(d).splits);
+}
 
-int twg_token_logprobs(const twg_token_logprobs_t *d, void *, size_t, twg_stream_t stream) {
+int twg_token_logprobs(const twg_token_logprobs_t *d, void *scratch, size_t scratch_bytes, twg_stream_t stream) {
   int rc = check(d, false);
   if (rc <= 0) return rc;
+  const RowShape shape = shape_of(d);
+  if (shape.splits > 1) {
+    if (!scratch || scratch_bytes < scratch_of(d, shape.splits)) return TWG_E_SCRATCH_SMALL;
+    if (!aligned_to(scratch, 8)) return TWG_E_INVALID_ARG;
+  }
   if ((rc = ensure_init())) return rc;
   LogprobArgs a = args_of(d);
+  a.splits = shape.splits;
+  a.scratch = static_cast<uint64_t *>(scratch);
   a.logprob = d->logprob;
   a.entropy = d->entropy;
   a.row_max = d->row_max;
   a.row_sum = d->row_sum;
   a.top_logprobs = d->top_logprobs;
   a.top_ids = d->top_ids;
+  const hipStream_t s = nn_stream(stream);
   return nn_dispatch(d->dtype, [&](auto t) {
-    logprobs_rows<decltype(t)><<<(unsigned)d->rows, kThreads, 0, nn_stream(stream)>>>(a);
+    using T = decltype(t);
+    const unsigned grid = (unsigned)(d->rows * shape.splits);
+    if (shape.waves == 1 && a.top_k)
+      logprobs_rows<T, 1, true><<<grid, 64, 0, s>>>(a);
+    else if (shape.waves == 1)
+      logprobs_rows<T, 1, false><<<grid, 64, 0, s>>>(a);
+    else if (a.top_k)
+      logprobs_rows<T, 4, true><<<grid, 256, 0, s>>>(a);
+    else
+      logprobs_rows<T, 4, false><<<grid, 256, 0, s>>>(a);
+    if (shape.splits > 1) logprobs_join<T><<<(unsigned)d->rows, kThreads, 0, s>>>(a);
     return (int)hipGetLastError();
   });
 }
