@@ -12,6 +12,7 @@ namespace twg {
 namespace {
 
 constexpr int kPer = 8;  // elements per Philox call, 16 bits each
+constexpr int kDenseThreads = 64;
 
 struct Words {
   uint32_t w[4];
@@ -73,10 +74,99 @@ __global__ void __launch_bounds__(kThreads) dropout_any(T *out, const T *x, cons
   }
 }
 
+// Rows whose elements lie side by side, whole groups of 8 and aligned to 16 bytes in every
+// operand: packs of 16 bytes.  DENSE: one long row, the last group of which may be short.
+// Bound by memory (2 or 3 x 8 elements per lane against ten rounds of two products): one group
+// per lane and no loop, as for the framework's other dense kernels.
+template <typename T, bool RES, bool DENSE, bool STREAM>
+__global__ void __launch_bounds__(kDenseThreads) dropout_packs(T *out, const T *x, const T *res, Geom g, DropArgs a) {
+  constexpr int E = 16 / (int)sizeof(T), P = kPer / E;
+  typedef Pack<T, E> Vec;
+  const int64_t group = (int64_t)blockIdx.x * kDenseThreads + threadIdx.x;
+  const int64_t e = group * kPer;
+  if (e >= g.numel) return;
+  int64_t oo = e, ox = e, orr = e;
+  if constexpr (!DENSE) {
+    int64_t rest = e / g.shape[0], i = e - rest * g.shape[0];
+    oo = ox = orr = i;
+    for (int d = 1; d < g.ndim; ++d) {
+      const int64_t q = rest / g.shape[d];
+      i = rest - q * g.shape[d];
+      rest = q;
+      oo += i * g.stride[TWG_OUT][d];
+      ox += i * g.stride[TWG_A][d];
+      if (RES) orr += i * g.stride[TWG_B][d];
+    }
+  }
+  const int count = DENSE && g.numel - e < kPer ? (int)(g.numel - e) : kPer;
+  Pack<T, kPer> vx, vr, vo;
+  if (count == kPer) {
+#pragma unroll
+    for (int p = 0; p < P; ++p) {
+      const Vec l = load_pack<STREAM>(reinterpret_cast<const Vec *>(x + ox) + p);
+      __builtin_memcpy(&vx.v[p * E], &l, 16);
+      if (RES) {
+        const Vec m = load_pack<STREAM>(reinterpret_cast<const Vec *>(res + orr) + p);
+        __builtin_memcpy(&vr.v[p * E], &m, 16);
+      }
+    }
+  } else {
+    for (int j = 0; j < count; ++j) {
+      vx.v[j] = x[ox + j];
+      if (RES) vr.v[j] = res[orr + j];
+    }
+  }
+  const Words w = philox((uint64_t)group, total_offset(a), a.seed);
+#pragma unroll
+  for (int j = 0; j < kPer; ++j) {
+    const uint32_t bits = (w.w[j / 2] >> (16 * (j & 1))) & 0xFFFFu;
+    vo.v[j] = (T)dropped((float)vx.v[j], RES ? (float)vr.v[j] : 0.0f, bits, a);
+  }
+  if (count == kPer) {
+#pragma unroll
+    for (int p = 0; p < P; ++p) {
+      Vec l;
+      __builtin_memcpy(&l, &vo.v[p * E], 16);
+      store_pack<STREAM>(reinterpret_cast<Vec *>(out + oo) + p, l);
+    }
+  } else {
+    for (int j = 0; j < count; ++j) out[oo + j] = vo.v[j];
+  }
+}
+
+// Whether every operand's groups of 8 elements are two or one aligned packs.
+bool packs_fit(const Geom &g, const void *out, const void *x, const void *res, int size) {
+  if (!aligned_to(out, 16) || !aligned_to(x, 16) || !aligned_to(res, 16)) return false;
+  const int ops = res ? 3 : 2;
+  for (int o = 0; o < ops; ++o) {
+    if (g.ndim && g.stride[o][0] != 1) return false;
+    for (int d = 1; d < g.ndim; ++d)
+      if (g.stride[o][d] * size % 16) return false;
+  }
+  return g.ndim <= 1 || g.shape[0] % kPer == 0;
+}
+
 template <typename T>
 int launch_dropout(T *out, const T *x, const T *res, const Geom &g, const DropArgs &a, hipStream_t s) {
   const int64_t groups = (g.numel + kPer - 1) / kPer, blocks = (groups + kThreads - 1) / kThreads;
   if (blocks > INT32_MAX) return TWG_E_TOO_LARGE;
+  if (packs_fit(g, out, x, res, (int)sizeof(T))) {
+    const int64_t small = (groups + kDenseThreads - 1) / kDenseThreads;
+    if (small > INT32_MAX) return TWG_E_TOO_LARGE;
+    const bool stream = g.numel * (int64_t)sizeof(T) * (res ? 3 : 2) > kStreamBytes, dense = g.ndim <= 1;
+#define TWG_DROP(RES, DENSE, STREAM) \
+  dropout_packs<T, RES, DENSE, STREAM><<<(unsigned)small, kDenseThreads, 0, s>>>(out, x, res, g, a)
+    if (res && dense && stream) TWG_DROP(true, true, true);
+    else if (res && dense) TWG_DROP(true, true, false);
+    else if (res && stream) TWG_DROP(true, false, true);
+    else if (res) TWG_DROP(true, false, false);
+    else if (dense && stream) TWG_DROP(false, true, true);
+    else if (dense) TWG_DROP(false, true, false);
+    else if (stream) TWG_DROP(false, false, true);
+    else TWG_DROP(false, false, false);
+#undef TWG_DROP
+    return (int)hipGetLastError();
+  }
   if (res)
     dropout_any<T, true><<<(unsigned)blocks, kThreads, 0, s>>>(out, x, res, g, a);
   else
