@@ -433,8 +433,14 @@ __global__ void __launch_bounds__(kThreads) logprobs_join(LogprobArgs a) {
   if (lane < k) put_top(a, row, lane, mine, st);
 }
 
-template <typename T>
+constexpr int kGradPacks = 2;  // packs of 16 bytes per lane
+
+// One workgroup: a stretch of one row.  What the elements share is the same for the whole
+// workgroup; each element costs one exponential.
+template <typename T, bool STREAM>
 __global__ void __launch_bounds__(kThreads) logprobs_grad(LogprobArgs a) {
+  constexpr int E = 16 / (int)sizeof(T), PER = kGradPacks * kThreads;
+  typedef Pack<T, E> Vec;
   const int64_t row = blockIdx.x;
   const T *x = (const T *)a.logits + row * a.row_stride;
   T *grad = (T *)a.grad + row * a.grad_stride;
@@ -445,16 +451,48 @@ __global__ void __launch_bounds__(kThreads) logprobs_grad(LogprobArgs a) {
   const float s = a.in_sum[row], m = a.in_max[row];
   if (!ignored && g_lp != 0.0f && (t < 0 || t >= a.vocab)) g_lp = __uint_as_float(0x7FC00000u);
   const bool none = (g_lp == 0.0f && g_h == 0.0f) || s == 0.0f;
-  const float c2 = a.scale * kLog2e, inv_s = 1.0f / s;
-  const float shift = g_h != 0.0f ? a.in_entropy[row] - logf(s) : 0.0f;
-  for (int j = blockIdx.y * kThreads + threadIdx.x; j < a.vocab; j += gridDim.y * kThreads) {
-    float g = 0.0f;
-    if (!none) {
-      const float d = ((float)x[j] - m) * c2, p = exp2_fast(d) * inv_s;
-      const float logs = __fmaf_rn(fmaxf(d, -300.0f), kLn2f, shift);
-      g = a.scale * ((j == t ? g_lp : 0.0f) - p * __fmaf_rn(g_h, logs, g_lp));
+  // grad = c [j = t] g_lp - 2^d (d h + l) with d = log2 e c (x - m), h = c g_H ln 2 / s,
+  // l = c (g_lp + g_H (entropy - log s)) / s
+  const float c2 = a.scale * kLog2e, by_s = a.scale / s, hit = a.scale * g_lp;
+  const float l = by_s * (g_h != 0.0f ? __fmaf_rn(g_h, a.in_entropy[row] - logf(s), g_lp) : g_lp);
+  const float h = by_s * g_h * kLn2f;
+  auto one = [&](float v, int j) {
+    const float d = (v - m) * c2, p = exp2_fast(d);
+    const float g = -p * __fmaf_rn(fmaxf(d, -300.0f), h, l);
+    return j == t ? g + hit : g;
+  };
+  // elements before the gradient's first 16-byte boundary, whole packs, elements behind them
+  const int lead = (int)((-(uintptr_t)grad & 15) / sizeof(T));
+  const int head = lead < a.vocab ? lead : a.vocab;
+  const int packs = (a.vocab - head) / E, tail = a.vocab - head - packs * E;
+  const bool alike = (((uintptr_t)x ^ (uintptr_t)grad) & 15) == 0;  // the logits' packs are aligned, too
+  for (int chunk = blockIdx.y; chunk * PER < packs || chunk == 0; chunk += gridDim.y) {
+    if (chunk == 0 && (int)threadIdx.x < head + tail) {
+      const int j = (int)threadIdx.x < head ? threadIdx.x : a.vocab - tail + (int)threadIdx.x - head;
+      grad[j] = (T)(none ? 0.0f : one((float)x[j], j));
     }
-    grad[j] = (T)g;
+    Vec v[kGradPacks];
+#pragma unroll
+    for (int u = 0; u < kGradPacks; ++u) {
+      const int p = chunk * PER + u * kThreads + threadIdx.x;
+      if (p >= packs || none) continue;
+      const T *from = x + head + p * E;
+      if (alike) {
+        v[u] = load_pack<STREAM>((const Vec *)from);
+      } else {
+#pragma unroll
+        for (int j = 0; j < E; ++j) v[u].v[j] = from[j];
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < kGradPacks; ++u) {
+      const int p = chunk * PER + u * kThreads + threadIdx.x;
+      if (p >= packs) continue;
+      Vec o;
+#pragma unroll
+      for (int j = 0; j < E; ++j) o.v[j] = (T)(none ? 0.0f : one((float)v[u].v[j], head + p * E + j));
+      store_pack<STREAM>((Vec *)(grad + head) + p, o);
+    }
   }
 }
 
@@ -580,9 +618,13 @@ int twg_token_logprobs_backward(const twg_token_logprobs_t *d, twg_stream_t stre
   a.grad = d->grad;
   a.grad_stride = d->grad_stride;
   return nn_dispatch(d->dtype, [&](auto t) {
-    const unsigned chunks = (unsigned)((d->vocab + 16 * kThreads - 1) / (16 * kThreads));
-    logprobs_grad<decltype(t)><<<dim3((unsigned)d->rows, chunks < 65535 ? chunks : 65535), kThreads, 0,
-                                 nn_stream(stream)>>>(a);
+    using T = decltype(t);
+    const int64_t per = kGradPacks * kThreads * 16 / (int)sizeof(T), chunks = (d->vocab + per - 1) / per;
+    const dim3 grid((unsigned)d->rows, (unsigned)(chunks < 65535 ? chunks : 65535));
+    if (2.0 * (double)d->rows * (double)d->vocab * sizeof(T) > (double)kStreamBytes)
+      logprobs_grad<T, true><<<grid, kThreads, 0, nn_stream(stream)>>>(a);
+    else
+      logprobs_grad<T, false><<<grid, kThreads, 0, nn_stream(stream)>>>(a);
     return (int)hipGetLastError();
   });
 }
