@@ -106,54 +106,137 @@ __device__ __forceinline__ void rotate(float *z, const float *cs, const float *s
   }
 }
 
+// Sum over the 2^log_g lanes of a group, the same bits in all of them.  Within 16 lanes by DPP:
+// neighbours, pairs, then mirrored halves and rows, whose members all hold their part's sum.
 __device__ __forceinline__ float group_sum(float v, int log_g) {
-  for (int i = 0; i < log_g; ++i) v += __shfl_xor(v, 1 << i);
+#define TWG_DPP(ctrl) __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), ctrl, 0xF, 0xF, false))
+  if (log_g > 0) v += TWG_DPP(0xB1);   // quad_perm 1 0 3 2
+  if (log_g > 1) v += TWG_DPP(0x4E);   // quad_perm 2 3 0 1
+  if (log_g > 2) v += TWG_DPP(0x141);  // row_half_mirror
+  if (log_g > 3) v += TWG_DPP(0x140);  // row_mirror
+#undef TWG_DPP
+  if (log_g > 4) v += __shfl_xor(v, 16);
+  if (log_g > 5) v += __shfl_xor(v, 32);
   return v;
 }
 
-// cosines and sines of tokens t0 .. t0 + tile - 1 into LDS
-__device__ __forceinline__ void fill_trig(const RopeArgs &a, int64_t t0, int n, float *cs, float *sn) {
+// What the heads of a token share: its angles' cosines and sines, and where it starts in the
+// inputs and results.
+struct TokenRoom {
+  float cs[kTrigRoom], sn[kTrigRoom];
+  int64_t x[kMaxTile][2], dy[kMaxTile][2], out[kMaxTile][2];
+};
+
+__device__ __forceinline__ void fill(const RopeArgs &a, uint32_t t0, int n, TokenRoom &room) {
+  const uint32_t tokens = (uint32_t)a.tokens;
   for (int i = threadIdx.x; i < n * a.rot_pairs; i += kThreads) {
-    const int lt = i / a.rot_pairs, p = i - lt * a.rot_pairs;
-    const int64_t tok = t0 + lt, b = tok / a.tokens, t = tok - b * a.tokens;
+    const uint32_t lt = (uint32_t)i / (uint32_t)a.rot_pairs, p = i - lt * a.rot_pairs;
+    const uint32_t b = (t0 + lt) / tokens, t = t0 + lt - b * tokens;
     float c, s;
     turn(position_at(a, a.pair_axis[p], b, t), a.inv_freq[p], &c, &s);
-    cs[i] = c;
-    sn[i] = s;
+    room.cs[i] = c;
+    room.sn[i] = s;
+  }
+  if ((int)threadIdx.x < 2 * n) {
+    const int lt = threadIdx.x >> 1, k = threadIdx.x & 1;
+    const uint32_t b = (t0 + lt) / tokens, t = t0 + lt - b * tokens;
+    room.x[lt][k] = b * a.part[k].xs[0] + t * a.part[k].xs[1];
+    room.dy[lt][k] = b * a.part[k].ys[0] + t * a.part[k].ys[1];
+    room.out[lt][k] = b * a.part[k].os[0] + t * a.part[k].os[1];
+  }
+}
+
+// The heads of a tile, token after token, dealt to the groups: head `h` of token `lt`, stepping on
+// by the number of groups.
+struct Place {
+  int lt, h;
+  __device__ __forceinline__ void step(int by, int heads) {
+    h += by;
+    while (h >= heads) {
+      h -= heads;
+      ++lt;
+    }
+  }
+};
+
+// A lane's V pairs of a head as they lie in memory: two runs of V elements.
+template <typename T, int V, int C>
+struct Raw {
+  Pack<T, V> v[C][2];
+};
+
+template <typename T, int V, int C, bool ADJ>
+__device__ __forceinline__ void fetch(const RopeArgs &a, const T *from, int lane, Raw<T, V, C> &to) {
+#pragma unroll
+  for (int c = 0; c < C; ++c) {
+    const int p0 = ((c << a.log_g) + lane) * V;
+    if (p0 < a.pairs) {
+      int first, second;
+      runs_of<V, ADJ>(a, p0, &first, &second);
+      to.v[c][0] = load_pack<false>((const Pack<T, V> *)(from + first));
+      to.v[c][1] = load_pack<false>((const Pack<T, V> *)(from + second));
+    }
+  }
+}
+
+// The lane's elements of a norm weight; ones without it.
+template <typename TW, int V, int C, bool ADJ>
+__device__ __forceinline__ void fetch_weight(const RopeArgs &a, int k, int lane, float (*w)[2 * V]) {
+  const TW *from = (const TW *)a.part[k].weight;
+#pragma unroll
+  for (int c = 0; c < C; ++c) {
+    const int p0 = ((c << a.log_g) + lane) * V;
+#pragma unroll
+    for (int j = 0; j < 2 * V; ++j) w[c][j] = 1.0f;
+    if (from && p0 < a.pairs) {
+      int first, second;
+      runs_of<V, ADJ>(a, p0, &first, &second);
+      load_run<TW, V>(w[c], from + first);
+      load_run<TW, V>(w[c] + V, from + second);
+    }
   }
 }
 
 // One workgroup: `tile` tokens, their heads dealt to groups of 2^log_g lanes; a lane holds V
-// pairs in each of C chunks of a head.
+// pairs in each of C chunks of a head.  A group's next head is on its way while it works
+// on one; the first is fetched before the angles are computed.
 template <typename T, typename TW, int V, int C, bool ADJ>
 __global__ void __launch_bounds__(kThreads) rope_forward(RopeArgs a) {
-  __shared__ float cs[kTrigRoom], sn[kTrigRoom];
-  const int64_t t0 = (int64_t)blockIdx.x * a.tile;
-  const int n = (int)min((int64_t)a.tile, a.all_tokens - t0);
-  fill_trig(a, t0, n, cs, sn);
+  __shared__ TokenRoom room;
+  const uint32_t t0 = blockIdx.x * (uint32_t)a.tile;
+  const int n = min(a.tile, (int)(a.all_tokens - t0));
+  const int lane = threadIdx.x & ((1 << a.log_g) - 1), groups = (kThreads >> a.log_g) * gridDim.y;
+  fill(a, t0, n, room);
+  float w[2][C][2 * V];
+  if (a.norm) {
+    fetch_weight<TW, V, C, ADJ>(a, 0, lane, w[0]);
+    fetch_weight<TW, V, C, ADJ>(a, 1, lane, w[1]);
+  }
   __syncthreads();
-  const int lane = threadIdx.x & ((1 << a.log_g) - 1), group = threadIdx.x >> a.log_g;
-  const int groups = (kThreads >> a.log_g) * gridDim.y;
-  for (int u = blockIdx.y * (kThreads >> a.log_g) + group; u < n * a.heads; u += groups) {
-    const int lt = u / a.heads;
-    int h = u - lt * a.heads;
-    const PartArgs &part = a.part[h >= a.heads0];
-    h -= h >= a.heads0 ? a.heads0 : 0;
-    const int64_t b = (t0 + lt) / a.tokens, t = t0 + lt - b * a.tokens;
-    const T *x = (const T *)part.x + b * part.xs[0] + t * part.xs[1] + h * part.xs[2];
-    T *out = (T *)part.out + b * part.os[0] + t * part.os[1] + h * part.os[2];
+  Place at{0, 0};
+  at.step((int)(blockIdx.y * (kThreads >> a.log_g) + (threadIdx.x >> a.log_g)), a.heads);
+  auto source = [&](const Place &q) {
+    const int k = q.h >= a.heads0;
+    return (const T *)a.part[k].x + room.x[q.lt][k] + (q.h - (k ? a.heads0 : 0)) * a.part[k].xs[2];
+  };
+  Raw<T, V, C> next;
+  if (at.lt < n) fetch<T, V, C, ADJ>(a, source(at), lane, next);
+  while (at.lt < n) {
+    const Raw<T, V, C> x = next;
+    const Place here = at;
+    at.step(groups, a.heads);
+    if (at.lt < n) fetch<T, V, C, ADJ>(a, source(at), lane, next);
+    const int k = here.h >= a.heads0;
+    T *out = (T *)a.part[k].out + room.out[here.lt][k] + (here.h - (k ? a.heads0 : 0)) * a.part[k].os[2];
     float z[C][2 * V];
     float sq = 0.0f;
 #pragma unroll
     for (int c = 0; c < C; ++c) {
-      const int p0 = ((c << a.log_g) + lane) * V;
-      if (p0 < a.pairs) {
-        int first, second;
-        runs_of<V, ADJ>(a, p0, &first, &second);
-        load_run<T, V>(z[c], x + first);
-        load_run<T, V>(z[c] + V, x + second);
+      if (((c << a.log_g) + lane) * V >= a.pairs) continue;
 #pragma unroll
-        for (int j = 0; j < 2 * V; ++j) sq = __fmaf_rn(z[c][j], z[c][j], sq);
+      for (int j = 0; j < 2 * V; ++j) {
+        z[c][j] = (float)x.v[c][j / V].v[j % V];
+        sq = __fmaf_rn(z[c][j], z[c][j], sq);
       }
     }
     float r = 1.0f;
@@ -161,22 +244,17 @@ __global__ void __launch_bounds__(kThreads) rope_forward(RopeArgs a) {
 #pragma unroll
     for (int c = 0; c < C; ++c) {
       const int p0 = ((c << a.log_g) + lane) * V;
-      if (p0 < a.pairs) {
-        int first, second;
-        runs_of<V, ADJ>(a, p0, &first, &second);
-        if (a.norm) {
-          float w[2 * V];
-          if (part.weight) {
-            load_run<TW, V>(w, (const TW *)part.weight + first);
-            load_run<TW, V>(w + V, (const TW *)part.weight + second);
-          }
+      if (p0 >= a.pairs) continue;
+      int first, second;
+      runs_of<V, ADJ>(a, p0, &first, &second);
+      if (a.norm) {
 #pragma unroll
-          for (int j = 0; j < 2 * V; ++j) z[c][j] = z[c][j] * r * (part.weight ? w[j] : 1.0f);
-        }
-        if (p0 < a.rot_pairs) rotate<V, ADJ>(z[c], cs + lt * a.rot_pairs + p0, sn + lt * a.rot_pairs + p0, 1.0f);
-        store_run<T, V>(out + first, z[c]);
-        store_run<T, V>(out + second, z[c] + V);
+        for (int j = 0; j < 2 * V; ++j) z[c][j] = z[c][j] * r * (k ? w[1][c][j] : w[0][c][j]);
       }
+      if (p0 < a.rot_pairs)
+        rotate<V, ADJ>(z[c], room.cs + here.lt * a.rot_pairs + p0, room.sn + here.lt * a.rot_pairs + p0, 1.0f);
+      store_run<T, V>(out + first, z[c]);
+      store_run<T, V>(out + second, z[c] + V);
     }
   }
 }
@@ -185,49 +263,58 @@ __global__ void __launch_bounds__(kThreads) rope_forward(RopeArgs a) {
 // sums of dz u for the weights' gradients in registers until its last tile is done.
 template <typename T, typename TW, int V, int C, bool ADJ>
 __global__ void __launch_bounds__(kThreads) rope_backward(RopeArgs a) {
-  __shared__ float cs[kTrigRoom], sn[kTrigRoom];
+  __shared__ TokenRoom room;
   __shared__ float joined[2][2 * kMaxPairs];
-  const int lane = threadIdx.x & ((1 << a.log_g) - 1), group = threadIdx.x >> a.log_g;
-  const int groups = kThreads >> a.log_g;
-  float dw[2][C][2 * V];
+  const int lane = threadIdx.x & ((1 << a.log_g) - 1), groups = kThreads >> a.log_g;
+  float dw[2][C][2 * V], w[2][C][2 * V];
 #pragma unroll
   for (int k = 0; k < 2; ++k)
 #pragma unroll
     for (int c = 0; c < C; ++c)
 #pragma unroll
       for (int j = 0; j < 2 * V; ++j) dw[k][c][j] = 0.0f;
-  for (int64_t t0 = (int64_t)blockIdx.x * a.tile; t0 < a.all_tokens; t0 += (int64_t)gridDim.x * a.tile) {
-    const int n = (int)min((int64_t)a.tile, a.all_tokens - t0);
+  if (a.norm) {
+    fetch_weight<TW, V, C, ADJ>(a, 0, lane, w[0]);
+    fetch_weight<TW, V, C, ADJ>(a, 1, lane, w[1]);
+  }
+  for (int64_t start = (int64_t)blockIdx.x * a.tile; start < a.all_tokens; start += (int64_t)gridDim.x * a.tile) {
+    const uint32_t t0 = (uint32_t)start;
+    const int n = min(a.tile, (int)(a.all_tokens - start));
     __syncthreads();
-    fill_trig(a, t0, n, cs, sn);
+    fill(a, t0, n, room);
     __syncthreads();
-    for (int u = group; u < n * a.heads; u += groups) {
-      const int lt = u / a.heads;
-      int h = u - lt * a.heads;
-      const int which = h >= a.heads0;
-      const PartArgs &part = a.part[which];
-      h -= which ? a.heads0 : 0;
-      const int64_t b = (t0 + lt) / a.tokens, t = t0 + lt - b * a.tokens;
-      const T *x = (const T *)part.x + b * part.xs[0] + t * part.xs[1] + h * part.xs[2];
-      const T *dy = (const T *)part.dy + b * part.ys[0] + t * part.ys[1] + h * part.ys[2];
-      T *out = (T *)part.out + b * part.os[0] + t * part.os[1] + h * part.os[2];
+    Place at{0, 0};
+    at.step((int)(threadIdx.x >> a.log_g), a.heads);
+    Raw<T, V, C> next_x, next_y;
+    auto get = [&](const Place &q) {
+      const int k = q.h >= a.heads0;
+      const int64_t h = q.h - (k ? a.heads0 : 0);
+      fetch<T, V, C, ADJ>(a, (const T *)a.part[k].dy + room.dy[q.lt][k] + h * a.part[k].ys[2], lane, next_y);
+      if (a.norm) fetch<T, V, C, ADJ>(a, (const T *)a.part[k].x + room.x[q.lt][k] + h * a.part[k].xs[2], lane, next_x);
+    };
+    if (at.lt < n) get(at);
+    while (at.lt < n) {
+      const Raw<T, V, C> x = next_x, y = next_y;
+      const Place here = at;
+      at.step(groups, a.heads);
+      if (at.lt < n) get(at);
+      const int k = here.h >= a.heads0;
+      T *out = (T *)a.part[k].out + room.out[here.lt][k] + (here.h - (k ? a.heads0 : 0)) * a.part[k].os[2];
       float z[C][2 * V], g[C][2 * V];
       float sq = 0.0f, dot = 0.0f;
 #pragma unroll
       for (int c = 0; c < C; ++c) {
         const int p0 = ((c << a.log_g) + lane) * V;
-        if (p0 < a.pairs) {
-          int first, second;
-          runs_of<V, ADJ>(a, p0, &first, &second);
-          load_run<T, V>(g[c], dy + first);
-          load_run<T, V>(g[c] + V, dy + second);
-          if (p0 < a.rot_pairs)
-            rotate<V, ADJ>(g[c], cs + lt * a.rot_pairs + p0, sn + lt * a.rot_pairs + p0, -1.0f);
-          if (a.norm) {
-            load_run<T, V>(z[c], x + first);
-            load_run<T, V>(z[c] + V, x + second);
+        if (p0 >= a.pairs) continue;
 #pragma unroll
-            for (int j = 0; j < 2 * V; ++j) sq = __fmaf_rn(z[c][j], z[c][j], sq);
+        for (int j = 0; j < 2 * V; ++j) g[c][j] = (float)y.v[c][j / V].v[j % V];
+        if (p0 < a.rot_pairs)
+          rotate<V, ADJ>(g[c], room.cs + here.lt * a.rot_pairs + p0, room.sn + here.lt * a.rot_pairs + p0, -1.0f);
+        if (a.norm) {
+#pragma unroll
+          for (int j = 0; j < 2 * V; ++j) {
+            z[c][j] = (float)x.v[c][j / V].v[j % V];
+            sq = __fmaf_rn(z[c][j], z[c][j], sq);
           }
         }
       }
@@ -236,24 +323,14 @@ __global__ void __launch_bounds__(kThreads) rope_backward(RopeArgs a) {
         r = 1.0f / sqrtf(__fmaf_rn(group_sum(sq, a.log_g), a.inv_dim, a.eps));
 #pragma unroll
         for (int c = 0; c < C; ++c) {
-          const int p0 = ((c << a.log_g) + lane) * V;
-          if (p0 < a.pairs) {
-            int first, second;
-            runs_of<V, ADJ>(a, p0, &first, &second);
-            float w[2 * V];
-            if (part.weight) {
-              load_run<TW, V>(w, (const TW *)part.weight + first);
-              load_run<TW, V>(w + V, (const TW *)part.weight + second);
-            }
+          if (((c << a.log_g) + lane) * V >= a.pairs) continue;
 #pragma unroll
-            for (int j = 0; j < 2 * V; ++j) {
-              z[c][j] *= r;
-              const float m = g[c][j] * z[c][j];
-              if (which) dw[1][c][j] += m;
-              else dw[0][c][j] += m;
-              g[c][j] *= part.weight ? w[j] : 1.0f;
-              dot = __fmaf_rn(g[c][j], z[c][j], dot);
-            }
+          for (int j = 0; j < 2 * V; ++j) {
+            z[c][j] *= r;
+            if (k) dw[1][c][j] = __fmaf_rn(g[c][j], z[c][j], dw[1][c][j]);
+            else dw[0][c][j] = __fmaf_rn(g[c][j], z[c][j], dw[0][c][j]);
+            g[c][j] *= k ? w[1][c][j] : w[0][c][j];
+            dot = __fmaf_rn(g[c][j], z[c][j], dot);
           }
         }
         dot = group_sum(dot, a.log_g) * a.inv_dim;
@@ -261,16 +338,15 @@ __global__ void __launch_bounds__(kThreads) rope_backward(RopeArgs a) {
 #pragma unroll
       for (int c = 0; c < C; ++c) {
         const int p0 = ((c << a.log_g) + lane) * V;
-        if (p0 < a.pairs) {
-          int first, second;
-          runs_of<V, ADJ>(a, p0, &first, &second);
-          if (a.norm) {
+        if (p0 >= a.pairs) continue;
+        int first, second;
+        runs_of<V, ADJ>(a, p0, &first, &second);
+        if (a.norm) {
 #pragma unroll
-            for (int j = 0; j < 2 * V; ++j) g[c][j] = r * __fmaf_rn(-z[c][j], dot, g[c][j]);
-          }
-          store_run<T, V>(out + first, g[c]);
-          store_run<T, V>(out + second, g[c] + V);
+          for (int j = 0; j < 2 * V; ++j) g[c][j] = r * __fmaf_rn(-z[c][j], dot, g[c][j]);
         }
+        store_run<T, V>(out + first, g[c]);
+        store_run<T, V>(out + second, g[c] + V);
       }
     }
   }
@@ -308,19 +384,27 @@ __global__ void __launch_bounds__(kThreads) rope_backward(RopeArgs a) {
   for (int i = threadIdx.x; i < 2 * dim; i += kThreads) mine[i] = joined[i >= dim][i >= dim ? i - dim : i];
 }
 
-// Sum of the workgroups' partial rows: 64 columns per workgroup, 16 lanes down each column.
+// Sum of the workgroups' partial rows: 32 columns per workgroup, 32 lanes down each column with
+// eight rows on their way at a time.
 template <typename TW>
 __global__ void __launch_bounds__(1024) rope_weight_sum(const float *partial, int rows, int dim, TW *dw0, TW *dw1) {
-  __shared__ float part[16][64];
-  const int col = blockIdx.x * 64 + (threadIdx.x & 63), y = threadIdx.x >> 6;
-  float sum = 0.0f;
-  if (col < 2 * dim)
-    for (int r = y; r < rows; r += 16) sum += partial[(int64_t)r * 2 * dim + col];
-  part[y][threadIdx.x & 63] = sum;
+  __shared__ float part[32][33];
+  const int col = blockIdx.x * 32 + (threadIdx.x & 31), y = threadIdx.x >> 5;
+  float sum[8] = {};
+  if (col < 2 * dim) {
+    for (int r0 = y; r0 < rows; r0 += 8 * 32) {
+#pragma unroll
+      for (int u = 0; u < 8; ++u) {
+        const int r = r0 + u * 32;
+        sum[u] += r < rows ? partial[(int64_t)r * 2 * dim + col] : 0.0f;
+      }
+    }
+  }
+  part[y][threadIdx.x & 31] = ((sum[0] + sum[1]) + (sum[2] + sum[3])) + ((sum[4] + sum[5]) + (sum[6] + sum[7]));
   __syncthreads();
   if (y || col >= 2 * dim) return;
   double total = 0.0;
-  for (int i = 0; i < 16; ++i) total += (double)part[i][threadIdx.x];
+  for (int i = 0; i < 32; ++i) total += (double)part[i][threadIdx.x];
   TW *to = col < dim ? dw0 : dw1;
   if (to) to[col < dim ? col : col - dim] = (TW)(float)total;
 }
@@ -503,7 +587,7 @@ int run(const twg_norm_rope_t *d, bool backward, void *scratch, size_t scratch_b
   return nn_dispatch(d->weight_dtype, [&](auto t) {
     using TW = decltype(t);
     const auto to = [&](int k) { return d->part[k].heads ? static_cast<TW *>(d->part[k].dweight) : nullptr; };
-    rope_weight_sum<TW><<<(2 * d->head_dim + 63) / 64, 1024, 0, s>>>(static_cast<const float *>(scratch), rows,
+    rope_weight_sum<TW><<<(2 * d->head_dim + 31) / 32, 1024, 0, s>>>(static_cast<const float *>(scratch), rows,
                                                                      d->head_dim, to(0), to(1));
     return (int)hipGetLastError();
   });
