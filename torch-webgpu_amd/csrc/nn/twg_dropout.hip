@@ -111,7 +111,9 @@ __global__ void __launch_bounds__(kDenseThreads) dropout_packs(T *out, const T *
       }
     }
   } else {
-    for (int j = 0; j < count; ++j) {
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) {
+      if (j >= count) continue;
       vx.v[j] = x[ox + j];
       if (RES) vr.v[j] = res[orr + j];
     }
@@ -130,7 +132,9 @@ __global__ void __launch_bounds__(kDenseThreads) dropout_packs(T *out, const T *
       store_pack<STREAM>(reinterpret_cast<Vec *>(out + oo) + p, l);
     }
   } else {
-    for (int j = 0; j < count; ++j) out[oo + j] = vo.v[j];
+#pragma unroll
+    for (int j = 0; j < kPer; ++j)
+      if (j < count) out[oo + j] = vo.v[j];
   }
 }
 

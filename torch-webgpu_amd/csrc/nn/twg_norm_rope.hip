@@ -16,25 +16,30 @@ constexpr int kMaxPairs = TWG_ROPE_MAX_HEAD_DIM / 2;
 constexpr int kTrigRoom = 1024;  // cosines (and sines) a workgroup holds: 8 KiB of LDS
 constexpr int kMaxTile = 16;     // tokens a workgroup takes at most
 
+// Queries and keys are two parts, each with workgroups of its own: what differs between the parts
+// is the same for a whole workgroup.
 struct PartArgs {
   const void *x, *dy, *weight;
   void *out;
+  float *partial;               // backward: [grid][head_dim] sums of dz u, or NULL
   int64_t xs[3], ys[3], os[3];  // batch, token, head
+  int32_t heads;
+  int32_t tile;   // tokens of one piece of work
+  int32_t split;  // pieces that share a tile's heads
+  int32_t work;   // pieces
+  int32_t grid;   // workgroups: piece i, i + grid, ... are one workgroup's
 };
 
 struct RopeArgs {
   int32_t pairs, rot_pairs;  // head_dim / 2, rot_dim / 2
-  int32_t heads0, heads;     // of part 0, of both
-  int32_t tile;              // tokens per workgroup
   int32_t log_g;             // log2 of the lanes per head
   int32_t position_dtype;
   int32_t norm;
   float eps, inv_dim;
-  int64_t all_tokens, tokens;  // batch * tokens, tokens of one sequence
+  uint32_t all_tokens, tokens;  // batch * tokens, tokens of one sequence
   int64_t pos_stride[3];
   const void *positions;
   const float *inv_freq;
-  float *partial;  // backward: [workgroup][2][head_dim] sums of dz u, or NULL
   PartArgs part[2];
   uint8_t pair_axis[kMaxPairs];
 };
@@ -124,39 +129,50 @@ __device__ __forceinline__ float group_sum(float v, int log_g) {
 // inputs and results.
 struct TokenRoom {
   float cs[kTrigRoom], sn[kTrigRoom];
-  int64_t x[kMaxTile][2], dy[kMaxTile][2], out[kMaxTile][2];
+  int64_t x[kMaxTile], dy[kMaxTile], out[kMaxTile];
 };
 
-__device__ __forceinline__ void fill(const RopeArgs &a, uint32_t t0, int n, TokenRoom &room) {
-  const uint32_t tokens = (uint32_t)a.tokens;
+__device__ __forceinline__ void fill(const RopeArgs &a, const PartArgs &part, uint32_t t0, int n, TokenRoom &room) {
   for (int i = threadIdx.x; i < n * a.rot_pairs; i += kThreads) {
     const uint32_t lt = (uint32_t)i / (uint32_t)a.rot_pairs, p = i - lt * a.rot_pairs;
-    const uint32_t b = (t0 + lt) / tokens, t = t0 + lt - b * tokens;
+    const uint32_t b = (t0 + lt) / a.tokens, t = t0 + lt - b * a.tokens;
     float c, s;
     turn(position_at(a, a.pair_axis[p], b, t), a.inv_freq[p], &c, &s);
     room.cs[i] = c;
     room.sn[i] = s;
   }
-  if ((int)threadIdx.x < 2 * n) {
-    const int lt = threadIdx.x >> 1, k = threadIdx.x & 1;
-    const uint32_t b = (t0 + lt) / tokens, t = t0 + lt - b * tokens;
-    room.x[lt][k] = b * a.part[k].xs[0] + t * a.part[k].xs[1];
-    room.dy[lt][k] = b * a.part[k].ys[0] + t * a.part[k].ys[1];
-    room.out[lt][k] = b * a.part[k].os[0] + t * a.part[k].os[1];
+  if ((int)threadIdx.x < n) {
+    const uint32_t b = (t0 + threadIdx.x) / a.tokens, t = t0 + threadIdx.x - b * a.tokens;
+    room.x[threadIdx.x] = b * part.xs[0] + t * part.xs[1];
+    room.dy[threadIdx.x] = b * part.ys[0] + t * part.ys[1];
+    room.out[threadIdx.x] = b * part.os[0] + t * part.os[1];
   }
 }
 
-// The heads of a tile, token after token, dealt to the groups: head `h` of token `lt`, stepping on
-// by the number of groups.
-struct Place {
-  int lt, h;
-  __device__ __forceinline__ void step(int by, int heads) {
-    h += by;
-    while (h >= heads) {
+// A piece of work: tokens t0 .. t0 + n - 1, of whose heads (token after token) a group takes
+// every step-th, starting with head `h` of token `lt`.
+struct Piece {
+  uint32_t t0;
+  int n, lt, h, by, heads;
+  __device__ __forceinline__ Piece(const RopeArgs &a, const PartArgs &part, int index) {
+    const int tile = index / part.split, share = index - tile * part.split, groups = kThreads >> a.log_g;
+    t0 = (uint32_t)tile * (uint32_t)part.tile;
+    n = (int)min((uint32_t)part.tile, a.all_tokens - t0);
+    heads = part.heads;
+    by = groups * part.split;
+    lt = 0;
+    h = 0;
+    step(share * groups + (int)(threadIdx.x >> a.log_g));
+  }
+  __device__ __forceinline__ void step(int k) {
+    h += k;
+    while (h >= heads && lt < n) {
       h -= heads;
       ++lt;
     }
   }
+  __device__ __forceinline__ void next() { step(by); }
+  __device__ __forceinline__ bool more() const { return lt < n; }
 };
 
 // A lane's V pairs of a head as they lie in memory: two runs of V elements.
@@ -166,7 +182,8 @@ struct Raw {
 };
 
 template <typename T, int V, int C, bool ADJ>
-__device__ __forceinline__ void fetch(const RopeArgs &a, const T *from, int lane, Raw<T, V, C> &to) {
+__device__ __forceinline__ void fetch(const RopeArgs &a, const void *base, int64_t offset, int lane, Raw<T, V, C> &to) {
+  const T *from = (const T *)base + offset;
 #pragma unroll
   for (int c = 0; c < C; ++c) {
     const int p0 = ((c << a.log_g) + lane) * V;
@@ -181,8 +198,8 @@ __device__ __forceinline__ void fetch(const RopeArgs &a, const T *from, int lane
 
 // The lane's elements of a norm weight; ones without it.
 template <typename TW, int V, int C, bool ADJ>
-__device__ __forceinline__ void fetch_weight(const RopeArgs &a, int k, int lane, float (*w)[2 * V]) {
-  const TW *from = (const TW *)a.part[k].weight;
+__device__ __forceinline__ void fetch_weight(const RopeArgs &a, const PartArgs &part, int lane, float (*w)[2 * V]) {
+  const TW *from = (const TW *)part.weight;
 #pragma unroll
   for (int c = 0; c < C; ++c) {
     const int p0 = ((c << a.log_g) + lane) * V;
@@ -197,37 +214,27 @@ __device__ __forceinline__ void fetch_weight(const RopeArgs &a, int k, int lane,
   }
 }
 
-// One workgroup: `tile` tokens, their heads dealt to groups of 2^log_g lanes; a lane holds V
-// pairs in each of C chunks of a head.  A group's next head is on its way while it works
-// on one; the first is fetched before the angles are computed.
+// A group of 2^log_g lanes works on one head at a time, a lane on V pairs in each of C chunks of
+// it.  The group's next head is on its way meanwhile.
 template <typename T, typename TW, int V, int C, bool ADJ>
 __global__ void __launch_bounds__(kThreads) rope_forward(RopeArgs a) {
   __shared__ TokenRoom room;
-  const uint32_t t0 = blockIdx.x * (uint32_t)a.tile;
-  const int n = min(a.tile, (int)(a.all_tokens - t0));
-  const int lane = threadIdx.x & ((1 << a.log_g) - 1), groups = (kThreads >> a.log_g) * gridDim.y;
-  fill(a, t0, n, room);
-  float w[2][C][2 * V];
-  if (a.norm) {
-    fetch_weight<TW, V, C, ADJ>(a, 0, lane, w[0]);
-    fetch_weight<TW, V, C, ADJ>(a, 1, lane, w[1]);
-  }
+  const bool second_part = (int)blockIdx.x >= a.part[0].grid;
+  const PartArgs &part = a.part[second_part];
+  const int lane = threadIdx.x & ((1 << a.log_g) - 1);
+  Piece at(a, part, (int)blockIdx.x - (second_part ? a.part[0].grid : 0));
+  fill(a, part, at.t0, at.n, room);
+  float w[C][2 * V];
+  if (a.norm) fetch_weight<TW, V, C, ADJ>(a, part, lane, w);
   __syncthreads();
-  Place at{0, 0};
-  at.step((int)(blockIdx.y * (kThreads >> a.log_g) + (threadIdx.x >> a.log_g)), a.heads);
-  auto source = [&](const Place &q) {
-    const int k = q.h >= a.heads0;
-    return (const T *)a.part[k].x + room.x[q.lt][k] + (q.h - (k ? a.heads0 : 0)) * a.part[k].xs[2];
-  };
-  Raw<T, V, C> next;
-  if (at.lt < n) fetch<T, V, C, ADJ>(a, source(at), lane, next);
-  while (at.lt < n) {
-    const Raw<T, V, C> x = next;
-    const Place here = at;
-    at.step(groups, a.heads);
-    if (at.lt < n) fetch<T, V, C, ADJ>(a, source(at), lane, next);
-    const int k = here.h >= a.heads0;
-    T *out = (T *)a.part[k].out + room.out[here.lt][k] + (here.h - (k ? a.heads0 : 0)) * a.part[k].os[2];
+  Raw<T, V, C> coming;
+  if (at.more()) fetch<T, V, C, ADJ>(a, part.x, room.x[at.lt] + at.h * part.xs[2], lane, coming);
+  while (at.more()) {
+    const Raw<T, V, C> x = coming;
+    const int lt = at.lt;
+    T *out = (T *)part.out + room.out[lt] + at.h * part.os[2];
+    at.next();
+    if (at.more()) fetch<T, V, C, ADJ>(a, part.x, room.x[at.lt] + at.h * part.xs[2], lane, coming);
     float z[C][2 * V];
     float sq = 0.0f;
 #pragma unroll
@@ -249,57 +256,49 @@ __global__ void __launch_bounds__(kThreads) rope_forward(RopeArgs a) {
       runs_of<V, ADJ>(a, p0, &first, &second);
       if (a.norm) {
 #pragma unroll
-        for (int j = 0; j < 2 * V; ++j) z[c][j] = z[c][j] * r * (k ? w[1][c][j] : w[0][c][j]);
+        for (int j = 0; j < 2 * V; ++j) z[c][j] = z[c][j] * r * w[c][j];
       }
       if (p0 < a.rot_pairs)
-        rotate<V, ADJ>(z[c], room.cs + here.lt * a.rot_pairs + p0, room.sn + here.lt * a.rot_pairs + p0, 1.0f);
+        rotate<V, ADJ>(z[c], room.cs + lt * a.rot_pairs + p0, room.sn + lt * a.rot_pairs + p0, 1.0f);
       store_run<T, V>(out + first, z[c]);
       store_run<T, V>(out + second, z[c] + V);
     }
   }
 }
 
-// The same walk; a workgroup takes tiles blockIdx.x, blockIdx.x + gridDim.x, ... and keeps its
-// sums of dz u for the weights' gradients in registers until its last tile is done.
+// The same walk, over as many pieces as there are for the workgroup: its sums of dz u for the
+// weight's gradient stay in registers until the last one is done.
 template <typename T, typename TW, int V, int C, bool ADJ>
 __global__ void __launch_bounds__(kThreads) rope_backward(RopeArgs a) {
   __shared__ TokenRoom room;
-  __shared__ float joined[2][2 * kMaxPairs];
-  const int lane = threadIdx.x & ((1 << a.log_g) - 1), groups = kThreads >> a.log_g;
-  float dw[2][C][2 * V], w[2][C][2 * V];
+  __shared__ float joined[2 * kMaxPairs];
+  const bool second_part = (int)blockIdx.x >= a.part[0].grid;
+  const PartArgs &part = a.part[second_part];
+  const int block = (int)blockIdx.x - (second_part ? a.part[0].grid : 0);
+  const int lane = threadIdx.x & ((1 << a.log_g) - 1);
+  float dw[C][2 * V], w[C][2 * V];
 #pragma unroll
-  for (int k = 0; k < 2; ++k)
+  for (int c = 0; c < C; ++c)
 #pragma unroll
-    for (int c = 0; c < C; ++c)
-#pragma unroll
-      for (int j = 0; j < 2 * V; ++j) dw[k][c][j] = 0.0f;
-  if (a.norm) {
-    fetch_weight<TW, V, C, ADJ>(a, 0, lane, w[0]);
-    fetch_weight<TW, V, C, ADJ>(a, 1, lane, w[1]);
-  }
-  for (int64_t start = (int64_t)blockIdx.x * a.tile; start < a.all_tokens; start += (int64_t)gridDim.x * a.tile) {
-    const uint32_t t0 = (uint32_t)start;
-    const int n = min(a.tile, (int)(a.all_tokens - start));
+    for (int j = 0; j < 2 * V; ++j) dw[c][j] = 0.0f;
+  if (a.norm) fetch_weight<TW, V, C, ADJ>(a, part, lane, w);
+  for (int64_t piece = block; piece < part.work; piece += part.grid) {
+    Piece at(a, part, (int)piece);
     __syncthreads();
-    fill(a, t0, n, room);
+    fill(a, part, at.t0, at.n, room);
     __syncthreads();
-    Place at{0, 0};
-    at.step((int)(threadIdx.x >> a.log_g), a.heads);
-    Raw<T, V, C> next_x, next_y;
-    auto get = [&](const Place &q) {
-      const int k = q.h >= a.heads0;
-      const int64_t h = q.h - (k ? a.heads0 : 0);
-      fetch<T, V, C, ADJ>(a, (const T *)a.part[k].dy + room.dy[q.lt][k] + h * a.part[k].ys[2], lane, next_y);
-      if (a.norm) fetch<T, V, C, ADJ>(a, (const T *)a.part[k].x + room.x[q.lt][k] + h * a.part[k].xs[2], lane, next_x);
+    Raw<T, V, C> coming_x, coming_y;
+    auto get = [&]() {
+      fetch<T, V, C, ADJ>(a, part.dy, room.dy[at.lt] + at.h * part.ys[2], lane, coming_y);
+      if (a.norm) fetch<T, V, C, ADJ>(a, part.x, room.x[at.lt] + at.h * part.xs[2], lane, coming_x);
     };
-    if (at.lt < n) get(at);
-    while (at.lt < n) {
-      const Raw<T, V, C> x = next_x, y = next_y;
-      const Place here = at;
-      at.step(groups, a.heads);
-      if (at.lt < n) get(at);
-      const int k = here.h >= a.heads0;
-      T *out = (T *)a.part[k].out + room.out[here.lt][k] + (here.h - (k ? a.heads0 : 0)) * a.part[k].os[2];
+    if (at.more()) get();
+    while (at.more()) {
+      const Raw<T, V, C> x = coming_x, y = coming_y;
+      const int lt = at.lt;
+      T *out = (T *)part.out + room.out[lt] + at.h * part.os[2];
+      at.next();
+      if (at.more()) get();
       float z[C][2 * V], g[C][2 * V];
       float sq = 0.0f, dot = 0.0f;
 #pragma unroll
@@ -309,7 +308,7 @@ __global__ void __launch_bounds__(kThreads) rope_backward(RopeArgs a) {
 #pragma unroll
         for (int j = 0; j < 2 * V; ++j) g[c][j] = (float)y.v[c][j / V].v[j % V];
         if (p0 < a.rot_pairs)
-          rotate<V, ADJ>(g[c], room.cs + here.lt * a.rot_pairs + p0, room.sn + here.lt * a.rot_pairs + p0, -1.0f);
+          rotate<V, ADJ>(g[c], room.cs + lt * a.rot_pairs + p0, room.sn + lt * a.rot_pairs + p0, -1.0f);
         if (a.norm) {
 #pragma unroll
           for (int j = 0; j < 2 * V; ++j) {
@@ -327,9 +326,8 @@ __global__ void __launch_bounds__(kThreads) rope_backward(RopeArgs a) {
 #pragma unroll
           for (int j = 0; j < 2 * V; ++j) {
             z[c][j] *= r;
-            if (k) dw[1][c][j] = __fmaf_rn(g[c][j], z[c][j], dw[1][c][j]);
-            else dw[0][c][j] = __fmaf_rn(g[c][j], z[c][j], dw[0][c][j]);
-            g[c][j] *= k ? w[1][c][j] : w[0][c][j];
+            dw[c][j] = __fmaf_rn(g[c][j], z[c][j], dw[c][j]);
+            g[c][j] *= w[c][j];
             dot = __fmaf_rn(g[c][j], z[c][j], dot);
           }
         }
@@ -350,90 +348,73 @@ __global__ void __launch_bounds__(kThreads) rope_backward(RopeArgs a) {
       }
     }
   }
-  if (!a.partial) return;
+  if (!part.partial) return;
   // join the groups of each wavefront, then the wavefronts in their order
 #pragma unroll
-  for (int k = 0; k < 2; ++k)
+  for (int c = 0; c < C; ++c)
 #pragma unroll
-    for (int c = 0; c < C; ++c)
-#pragma unroll
-      for (int j = 0; j < 2 * V; ++j)
-        for (int i = a.log_g; i < 6; ++i) dw[k][c][j] += __shfl_xor(dw[k][c][j], 1 << i);
+    for (int j = 0; j < 2 * V; ++j)
+      for (int i = a.log_g; i < 6; ++i) dw[c][j] += __shfl_xor(dw[c][j], 1 << i);
   for (int wave = 0; wave < kThreads / 64; ++wave) {
     if ((int)(threadIdx.x >> 6) == wave && (int)(threadIdx.x & 63) < (1 << a.log_g)) {
 #pragma unroll
-      for (int k = 0; k < 2; ++k)
+      for (int c = 0; c < C; ++c) {
+        const int p0 = ((c << a.log_g) + lane) * V;
+        if (p0 < a.pairs) {
+          int first, second;
+          runs_of<V, ADJ>(a, p0, &first, &second);
 #pragma unroll
-        for (int c = 0; c < C; ++c) {
-          const int p0 = ((c << a.log_g) + lane) * V;
-          if (p0 < a.pairs) {
-            int first, second;
-            runs_of<V, ADJ>(a, p0, &first, &second);
-#pragma unroll
-            for (int j = 0; j < 2 * V; ++j) {
-              float &to = joined[k][j < V ? first + j : second + j - V];
-              to = wave ? to + dw[k][c][j] : dw[k][c][j];
-            }
+          for (int j = 0; j < 2 * V; ++j) {
+            float &to = joined[j < V ? first + j : second + j - V];
+            to = wave ? to + dw[c][j] : dw[c][j];
           }
         }
+      }
     }
     __syncthreads();
   }
   const int dim = 2 * a.pairs;
-  float *mine = a.partial + (int64_t)blockIdx.x * 2 * dim;
-  for (int i = threadIdx.x; i < 2 * dim; i += kThreads) mine[i] = joined[i >= dim][i >= dim ? i - dim : i];
+  for (int i = threadIdx.x; i < dim; i += kThreads) part.partial[(int64_t)block * dim + i] = joined[i];
 }
 
-// Sum of the workgroups' partial rows: 32 columns per workgroup, 32 lanes down each column with
-// eight rows on their way at a time.
+// Sum of the workgroups' partial rows, one part per grid row: 32 columns per workgroup, 32 lanes
+// down each column with eight rows on their way at a time.
+struct SumArgs {
+  const float *partial[2];
+  int32_t rows[2];
+  void *to[2];
+  int32_t dim;
+};
 template <typename TW>
-__global__ void __launch_bounds__(1024) rope_weight_sum(const float *partial, int rows, int dim, TW *dw0, TW *dw1) {
+__global__ void __launch_bounds__(1024) rope_weight_sum(SumArgs a) {
   __shared__ float part[32][33];
-  const int col = blockIdx.x * 32 + (threadIdx.x & 31), y = threadIdx.x >> 5;
+  const int k = blockIdx.y, col = blockIdx.x * 32 + (threadIdx.x & 31), y = threadIdx.x >> 5;
+  if (!a.to[k]) return;
+  const float *from = a.partial[k] + col;
   float sum[8] = {};
-  if (col < 2 * dim) {
-    for (int r0 = y; r0 < rows; r0 += 8 * 32) {
+  if (col < a.dim) {
+    for (int r0 = y; r0 < a.rows[k]; r0 += 8 * 32) {
 #pragma unroll
       for (int u = 0; u < 8; ++u) {
         const int r = r0 + u * 32;
-        sum[u] += r < rows ? partial[(int64_t)r * 2 * dim + col] : 0.0f;
+        sum[u] += r < a.rows[k] ? from[(int64_t)r * a.dim] : 0.0f;
       }
     }
   }
   part[y][threadIdx.x & 31] = ((sum[0] + sum[1]) + (sum[2] + sum[3])) + ((sum[4] + sum[5]) + (sum[6] + sum[7]));
   __syncthreads();
-  if (y || col >= 2 * dim) return;
+  if (y || col >= a.dim) return;
   double total = 0.0;
   for (int i = 0; i < 32; ++i) total += (double)part[i][threadIdx.x];
-  TW *to = col < dim ? dw0 : dw1;
-  if (to) to[col < dim ? col : col - dim] = (TW)(float)total;
+  ((TW *)a.to[k])[col] = (TW)(float)total;
 }
 
 // ------------------------------------------------------------------ host side
 
-constexpr int kMaxPartials = 1024;
-
 int64_t total_heads(const twg_norm_rope_t *d) { return d->part[0].heads + d->part[1].heads; }
 
-bool wants_dweight(const twg_norm_rope_t *d) {
-  return d->norm && ((d->part[0].heads && d->part[0].dweight) || (d->part[1].heads && d->part[1].dweight));
-}
-
-// tokens per workgroup: enough heads for its groups, as far as the cosines fit
-int tile_of(const twg_norm_rope_t *d, int64_t all_tokens) {
-  const int rot = d->rot_dim / 2 > 0 ? d->rot_dim / 2 : 1;
-  int tile = 1;
-  while (tile < kMaxTile && 2 * tile * rot <= kTrigRoom && tile * total_heads(d) < 128 &&
-         all_tokens / (2 * tile) >= 1024)
-    tile *= 2;
-  return tile;
-}
-
-int partial_rows(const twg_norm_rope_t *d) {
-  const int64_t all = d->batch * d->tokens;
-  const int64_t tiles = (all + tile_of(d, all) - 1) / tile_of(d, all);
-  return (int)(tiles < kMaxPartials ? tiles : kMaxPartials);
-}
+bool wants_dweight(const twg_norm_rope_t *d, int k) { return d->norm && d->part[k].heads && d->part[k].dweight; }
+bool wants_dweight(const twg_norm_rope_t *d) { return wants_dweight(d, 0) || wants_dweight(d, 1); }
 
 // 0 = nothing to do, 1 = go on, negative = refused
 int check(const twg_norm_rope_t *d, bool backward) {
@@ -491,8 +472,49 @@ bool runs_aligned(const twg_norm_rope_t *d, bool backward, int v) {
   return true;
 }
 
+// Elements of a run and lanes of a group: the widest runs that everything is aligned to, 16 bytes
+// of T where possible.
+struct Lanes {
+  int v, log_g;
+};
+Lanes lanes_of(const twg_norm_rope_t *d, bool backward) {
+  Lanes l{16 / nn_size(d->dtype), 0};
+  while (l.v > 1 && !runs_aligned(d, backward, l.v)) l.v /= 2;
+  while ((l.v << l.log_g) < d->head_dim / 2 && l.log_g < 6) ++l.log_g;
+  return l;
+}
+
+constexpr int kMaxSums = 1536;  // workgroups of one part that leave sums for the weight's gradient
+constexpr int kSteps = 4;       // heads a group takes in a piece of work where there are many
+
+// How a part is cut into pieces: as many tokens as give each group kSteps heads (one where there is
+// too little work to fill the chip with), or a share of one token's heads.
+void cut(const twg_norm_rope_t *d, bool backward, int k, PartArgs &p) {
+  const int64_t all = d->batch * d->tokens, heads = d->part[k].heads;
+  p.heads = (int32_t)heads;
+  p.tile = p.split = 1;
+  p.work = p.grid = 0;
+  if (!heads || !all) return;
+  const int groups = kThreads >> lanes_of(d, backward).log_g;
+  const int64_t passes = all * total_heads(d) / groups / 1024;
+  const int64_t want = groups * (passes < 1 ? 1 : passes < kSteps ? passes : kSteps);
+  const int rot = d->rot_dim > 2 ? d->rot_dim / 2 : 1;
+  int64_t tile = (want + heads - 1) / heads;
+  if (tile > kMaxTile) tile = kMaxTile;
+  if (tile > kTrigRoom / rot) tile = kTrigRoom / rot;
+  if (tile > all) tile = all;
+  const int64_t split = (tile * heads + want - 1) / want;
+  const int64_t tiles = (all + tile - 1) / tile;
+  p.tile = (int32_t)tile;
+  p.split = (int32_t)(tiles * split > INT32_MAX / 2 ? 1 : split);
+  p.work = (int32_t)(tiles * p.split);
+  p.grid = p.work;
+  if (backward && wants_dweight(d, k) && p.grid > kMaxSums) p.grid = kMaxSums;
+}
+
 template <typename T, typename TW, int V, int C, bool ADJ>
-int launch(const RopeArgs &a, bool backward, dim3 grid, hipStream_t s) {
+int launch(const RopeArgs &a, bool backward, hipStream_t s) {
+  const unsigned grid = (unsigned)(a.part[0].grid + a.part[1].grid);
   if (backward)
     rope_backward<T, TW, V, C, ADJ><<<grid, kThreads, 0, s>>>(a);
   else
@@ -501,29 +523,10 @@ int launch(const RopeArgs &a, bool backward, dim3 grid, hipStream_t s) {
 }
 
 template <typename T, typename TW>
-int launch_typed(const twg_norm_rope_t *d, RopeArgs a, bool backward, hipStream_t s) {
-  // the widest runs that everything is aligned to: 16 bytes of T where possible
-  constexpr int W = 16 / (int)sizeof(T);
-  const int v = runs_aligned(d, backward, W) ? W : runs_aligned(d, backward, 4) ? 4
-              : runs_aligned(d, backward, 2) ? 2 : 1;
-  const int lanes = (a.pairs + v - 1) / v;
-  a.log_g = 0;
-  while ((1 << a.log_g) < lanes && a.log_g < 6) ++a.log_g;
-  const int64_t tiles = (a.all_tokens + a.tile - 1) / a.tile;
-  dim3 grid((unsigned)tiles, 1);
-  if (backward) {
-    if (a.partial) grid.x = (unsigned)partial_rows(d);
-  } else {
-    // few tokens: their heads are spread over several workgroups, one head per group
-    const int64_t per_pass = kThreads >> a.log_g, units = (int64_t)a.tile * a.heads;
-    const int64_t split = (units + per_pass - 1) / per_pass;
-    while ((int64_t)grid.y * 2 <= split && tiles * grid.y < 1024) grid.y *= 2;
-  }
-  const bool adj = d->adjacent != 0;
-#define TWG_ROPE_V(V, C)                                                   \
-  (adj ? launch<T, TW, V, C, true>(a, backward, grid, s)                   \
-       : launch<T, TW, V, C, false>(a, backward, grid, s))
-  if constexpr (W == 8)
+int launch_typed(const RopeArgs &a, int v, bool adjacent, bool backward, hipStream_t s) {
+#define TWG_ROPE_V(V, C) \
+  (adjacent ? launch<T, TW, V, C, true>(a, backward, s) : launch<T, TW, V, C, false>(a, backward, s))
+  if constexpr (sizeof(T) == 2)
     if (v == 8) return TWG_ROPE_V(8, 1);
   if (v == 4) return TWG_ROPE_V(4, 1);
   if (v == 2) return TWG_ROPE_V(2, 2);
@@ -543,52 +546,59 @@ int run(const twg_norm_rope_t *d, bool backward, void *scratch, size_t scratch_b
   if (rc == 0 && !dw) return 0;
   if (int e = ensure_init()) return e;
   const hipStream_t s = nn_stream(stream);
-  int rows = 0;
+  SumArgs sums{};
+  sums.dim = d->head_dim;
+  for (int k = 0; k < 2; ++k) sums.to[k] = d->part[k].heads ? d->part[k].dweight : nullptr;
   if (rc > 0) {
     RopeArgs a{};
+    const Lanes lanes = lanes_of(d, backward);
     a.pairs = d->head_dim / 2;
     a.rot_pairs = d->rot_dim / 2;
-    a.heads0 = (int32_t)d->part[0].heads;
-    a.heads = (int32_t)total_heads(d);
-    a.all_tokens = d->batch * d->tokens;
-    a.tokens = d->tokens;
-    a.tile = tile_of(d, a.all_tokens);
+    a.log_g = lanes.log_g;
+    a.all_tokens = (uint32_t)(d->batch * d->tokens);
+    a.tokens = (uint32_t)d->tokens;
     a.position_dtype = d->position_dtype;
     a.norm = d->norm != 0;
     a.eps = d->eps;
     a.inv_dim = 1.0f / (float)d->head_dim;
     a.positions = d->positions;
     a.inv_freq = d->inv_freq;
-    a.partial = dw ? static_cast<float *>(scratch) : nullptr;
     for (int k = 0; k < 3; ++k) a.pos_stride[k] = d->pos_stride[k];
+    float *room = static_cast<float *>(scratch);
     for (int k = 0; k < 2; ++k) {
       const twg_rope_part_t &p = d->part[k];
-      a.part[k].x = p.x;
-      a.part[k].dy = p.dy;
-      a.part[k].weight = p.weight;
-      a.part[k].out = p.out;
+      PartArgs &to = a.part[k];
+      cut(d, backward, k, to);
+      to.x = p.x;
+      to.dy = p.dy;
+      to.weight = p.weight;
+      to.out = p.out;
+      if (backward && wants_dweight(d, k)) {
+        to.partial = room;
+        sums.partial[k] = room;
+        sums.rows[k] = to.grid;
+        room += (size_t)to.grid * (size_t)d->head_dim;
+      }
       for (int i = 0; i < 3; ++i) {
-        a.part[k].xs[i] = p.x_stride[i];
-        a.part[k].ys[i] = p.dy_stride[i];
-        a.part[k].os[i] = p.out_stride[i];
+        to.xs[i] = p.x_stride[i];
+        to.ys[i] = p.dy_stride[i];
+        to.os[i] = p.out_stride[i];
       }
     }
+    if ((int64_t)a.part[0].grid + a.part[1].grid > INT32_MAX) return TWG_E_TOO_LARGE;
     for (int i = 0; i < a.rot_pairs; ++i) a.pair_axis[i] = d->pair_axis[i];
     rc = nn_dispatch(d->dtype, [&](auto t) {
       using T = decltype(t);
       // weights come in the heads' type or in binary32
-      if (d->norm && d->weight_dtype == TWG_DT_F32) return launch_typed<T, float>(d, a, backward, s);
-      return launch_typed<T, T>(d, a, backward, s);
+      if (d->norm && d->weight_dtype == TWG_DT_F32)
+        return launch_typed<T, float>(a, lanes.v, d->adjacent != 0, backward, s);
+      return launch_typed<T, T>(a, lanes.v, d->adjacent != 0, backward, s);
     });
     if (rc) return rc;
-    rows = dw ? partial_rows(d) : 0;
   }
   if (!dw) return 0;
   return nn_dispatch(d->weight_dtype, [&](auto t) {
-    using TW = decltype(t);
-    const auto to = [&](int k) { return d->part[k].heads ? static_cast<TW *>(d->part[k].dweight) : nullptr; };
-    rope_weight_sum<TW><<<(2 * d->head_dim + 31) / 32, 1024, 0, s>>>(static_cast<const float *>(scratch), rows,
-                                                                     d->head_dim, to(0), to(1));
+    rope_weight_sum<decltype(t)><<<dim3((d->head_dim + 31) / 32, 2), 1024, 0, s>>>(sums);
     return (int)hipGetLastError();
   });
 }
@@ -608,7 +618,13 @@ int twg_norm_rope_backward(const twg_norm_rope_t *d, void *scratch, size_t scrat
 
 size_t twg_norm_rope_backward_scratch_bytes(const twg_norm_rope_t *d) {
   if (check(d, true) <= 0 || !wants_dweight(d)) return 0;
-  return (size_t)partial_rows(d) * 2 * (size_t)d->head_dim * sizeof(float);
+  size_t rows = 0;
+  for (int k = 0; k < 2; ++k) {
+    PartArgs p{};
+    cut(d, true, k, p);
+    if (wants_dweight(d, k)) rows += (size_t)p.grid;
+  }
+  return rows * (size_t)d->head_dim * sizeof(float);
 }
 
 }  // extern "C"
