@@ -210,14 +210,20 @@ struct BestList {
   }
 };
 
-// Of 64 lanes' values the k-th largest: every value's place by comparing it with all others.
+// A value that at least k lanes' values reach, and the upper half of the k-th largest of them: bit
+// by bit, the largest that k lanes still reach.
 __device__ __forceinline__ uint32_t kth_of_lanes(uint32_t v, int k) {
-  int above = 0;
-#pragma unroll
-  for (int i = 0; i < 64; ++i) above += (uint32_t)__builtin_amdgcn_readlane(v, i) > v;
-  uint32_t least = above < k ? v : 0xFFFFFFFFu;
-  for (int i = 1; i < 64; i <<= 1) least = min(least, (uint32_t)__shfl_xor((int)least, i));
-  return least;
+  uint32_t found = 0;
+  for (uint32_t bit = 0x80000000u; bit >= 0x10000u; bit >>= 1)
+    if (__popcll(__ballot(v >= (found | bit))) >= k) found |= bit;
+  return found;
+}
+
+// the larger of three in one instruction (fmaxf first makes sure of each operand)
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+  return r;
 }
 
 constexpr int kUnroll = 4;  // packs of 16 bytes a lane loads before it looks at the first
@@ -247,15 +253,9 @@ __global__ void __launch_bounds__(64 * WAVES) logprobs_rows(LogprobArgs a) {
   Run r{-INFINITY, 0.0f, 0.0f};
   float b = base_of(r.m, c2);
   BestList best{0, 0};
-  if (TOP && lane == 0) floors[wave] = 0;
-  if (TOP) __syncthreads();
 
-  // n values of this lane into its running sums
-  auto add = [&](const float *v, auto n) {
-    constexpr int COUNT = decltype(n)::value;
-    float top = v[0];
-#pragma unroll
-    for (int j = 1; j < COUNT; ++j) top = fmaxf(top, v[j]);
+  // n values of this lane, `top` the largest, into its running sums
+  auto add = [&](const float *v, float top, auto n) {
     if (top > r.m) {
       const float nb = base_of(top, c2), d = fmaxf(b - nb, -300.0f), f = exp2_fast(d);
       r.t = f * __fmaf_rn(d, r.s, r.t);
@@ -264,76 +264,96 @@ __global__ void __launch_bounds__(64 * WAVES) logprobs_rows(LogprobArgs a) {
       b = nb;
     }
 #pragma unroll
-    for (int j = 0; j < COUNT; ++j) {
+    for (int j = 0; j < decltype(n)::value; ++j) {
       const float d = __fmaf_rn(v[j], c2, -b), e = exp2_fast(d);
       r.s += e;
       r.t = __fmaf_rn(e, fmaxf(d, -300.0f), r.t);
     }
-    return top;
   };
   // the few single elements at an end of the row: the first lanes of the first wavefront
   auto edge = [&](int from, int n) {
     if (wave != 0 || n == 0) return;
     const bool has = lane < n;
     const float v = has ? (float)x[from + lane] : -INFINITY;
-    add(&v, std::integral_constant<int, 1>());
+    add(&v, v, std::integral_constant<int, 1>());
     if (TOP) best.insert(has ? key_of(v, (uint32_t)(from + lane)) : 0, k, lane);
   };
-
-  if (split == 0) edge(0, head);
-  for (int p = first; p < last; p += kUnroll * THREADS) {
+  // kUnroll packs of this lane, the first one pack `p` + threadIdx.x
+  uint32_t floor = 0;  // a rank that at least k elements of the row reach, as far as known
+  auto step = [&](int p, auto whole) {
     Pack<T, E> raw[kUnroll];
     bool in[kUnroll];
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u) {
       const int at = p + u * THREADS + (int)threadIdx.x;
-      in[u] = at < last;
+      in[u] = decltype(whole)::value || at < last;
       raw[u] = load_pack<true>(body + (in[u] ? at : last - 1));
     }
-    float v[N];
+    float v[N], most[kUnroll];
 #pragma unroll
-    for (int u = 0; u < kUnroll; ++u)
+    for (int u = 0; u < kUnroll; ++u) {
 #pragma unroll
       for (int j = 0; j < E; ++j) v[u * E + j] = in[u] ? (float)raw[u].v[j] : -INFINITY;
-    const float top = add(v, std::integral_constant<int, N>());
+      most[u] = max3(v[u * E], v[u * E + 1], v[u * E + 2]);
+#pragma unroll
+      for (int j = 3; j < E; j += 2) most[u] = max3(most[u], v[u * E + j], v[u * E + (j + 1 < E ? j + 1 : j)]);
+    }
+    const float top = max3(max3(most[0], most[1], most[2]), most[3], most[3]);
+    add(v, top, std::integral_constant<int, N>());
     if constexpr (TOP) {
-      // Which elements may be among the best.  An element of a later step has a higher id than
-      // everything in the list, so it has to be larger than the k-th.  At least k elements of the
-      // row are as large as the smallest of the wavefronts' `floors`, each the
-      // ceil(k / WAVES)-th best of its wavefront.  While the list is not full: at least k
-      // elements of this step are as large as the k-th largest of the lanes' maxima.
-      bool all = false;
-      uint32_t least;  // rank a candidate has to reach
-      if (best.kth == 0) {
-        least = kth_of_lanes(rank_of(top), k);
-        all = least == rank_of(-INFINITY);
-      } else {
-        least = (uint32_t)(best.kth >> 32) + 1;
+      // Which elements may be among the best k.  One of a later step has a higher id than all in
+      // the wavefront's list, so it has to be larger than a k-th there.  And at least k elements
+      // of the row reach `floor`, the smallest of the wavefronts' `floors`: in its first step
+      // each knows a value that ceil(k / WAVES) of its lanes' maxima reach, later the
+      // ceil(k / WAVES)-th of its list.
+      const uint32_t rank = rank_of(top);
+      if (p == first) {
+        const uint32_t mine = kth_of_lanes(rank, (k + WAVES - 1) / WAVES);
+        floor = mine;
+        if (WAVES > 1) {
+          if (lane == 0) floors[wave] = mine;
+          __syncthreads();
+        }
       }
       if (WAVES > 1) {
-        uint32_t floor = 0xFFFFFFFFu;
+        uint32_t all = 0xFFFFFFFFu;
 #pragma unroll
-        for (int w = 0; w < WAVES; ++w) floor = min(floor, __hip_atomic_load(&floors[w], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP));
-        least = max(least, floor);
+        for (int w = 0; w < WAVES; ++w)
+          all = min(all, __hip_atomic_load(&floors[w], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP));
+        floor = p == first ? all : max(floor, all);
       }
-      if (all || __ballot(rank_of(top) >= least)) {
-        // above the value one rank below `least` (that of -0, which 0x7FFFFFFF would be, is not in use)
-        const float bar = value_of_rank(least - (least == 0x80000000u ? 2 : 1));
+      const uint32_t least = max(floor, best.kth ? (uint32_t)(best.kth >> 32) + 1 : 0u);
+      if (__ballot(rank >= least)) {
+        // `any`: entries of -inf count, too.  Otherwise above the value one rank below `least` (0x7FFFFFFF,
+        // which would be -0, is not in use).
+        const bool any = least <= rank_of(-INFINITY);
+        const float bar = any ? -INFINITY : value_of_rank(least - (least == 0x80000000u ? 2 : 1));
 #pragma unroll
-        for (int j = 0; j < N; ++j) {
-          const bool cand = all ? in[j / E] : v[j] > bar;
-          if (__ballot(cand)) {
-            const uint32_t id = (uint32_t)(head + (p + (j / E) * THREADS + (int)threadIdx.x) * E + j % E);
-            best.insert(cand ? key_of(v[j], id) : 0, k, lane);
+        for (int u = 0; u < kUnroll; ++u) {
+          if (!any && !__ballot(most[u] > bar)) continue;
+#pragma unroll
+          for (int j = 0; j < E; ++j) {
+            const float e = v[u * E + j];
+            const bool cand = any ? in[u] : e > bar;
+            if (__ballot(cand)) {
+              const uint32_t id = (uint32_t)(head + (p + u * THREADS + (int)threadIdx.x) * E + j);
+              best.insert(cand ? key_of(e, id) : 0, k, lane);
+            }
           }
         }
         if (WAVES > 1) {
-          const uint64_t at = read_lane(best.mine, (k + WAVES - 1) / WAVES - 1);
-          if (lane == 0) __hip_atomic_store(&floors[wave], (uint32_t)(at >> 32), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+          const uint32_t at = (uint32_t)(read_lane(best.mine, (k + WAVES - 1) / WAVES - 1) >> 32);
+          if (lane == 0 && at > floors[wave])
+            __hip_atomic_store(&floors[wave], at, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
         }
       }
     }
-  }
+  };
+
+  if (split == 0) edge(0, head);
+  int p = first;
+  for (; p + kUnroll * THREADS <= last; p += kUnroll * THREADS) step(p, std::true_type());
+  if (p < last) step(p, std::false_type());
   if (split == a.splits - 1) edge(a.vocab - tail, tail);
 
   // join the lanes, then the wavefronts
