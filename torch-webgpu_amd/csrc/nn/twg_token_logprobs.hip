@@ -73,8 +73,39 @@ __device__ __forceinline__ Run join(const Run &a, const Run &b, float c2) {
   return Run{m, __fmaf_rn(f, ls, hs), __fmaf_rn(f, __fmaf_rn(d, ls, lt), ht)};
 }
 
-__device__ __forceinline__ Run shuffled(const Run &r, int lanes) {
-  return Run{__shfl_xor(r.m, lanes), __shfl_xor(r.s, lanes), __shfl_xor(r.t, lanes)};
+// One value from the 64 lanes' in all of them, by moves within rows of 16 lanes and across them
+// (DPP); `none` takes the place of lanes that a move does not reach.
+template <typename Op>
+__device__ __forceinline__ uint32_t over_lanes(uint32_t v, uint32_t none, Op op) {
+#define TWG_STEP(ctrl, rows) v = op(v, (uint32_t)__builtin_amdgcn_update_dpp((int)none, (int)v, ctrl, rows, 0xF, false))
+  TWG_STEP(0x111, 0xF);  // row_shr:1
+  TWG_STEP(0x112, 0xF);  // row_shr:2
+  TWG_STEP(0x114, 0xF);  // row_shr:4
+  TWG_STEP(0x118, 0xF);  // row_shr:8: lane 15 of each row has the row's
+  TWG_STEP(0x142, 0xA);  // row_bcast:15
+  TWG_STEP(0x143, 0xC);  // row_bcast:31: lane 63 has all
+#undef TWG_STEP
+  return (uint32_t)__builtin_amdgcn_readlane((int)v, 63);
+}
+__device__ __forceinline__ uint32_t max_of_lanes(uint32_t v) {
+  return over_lanes(v, 0, [](uint32_t a, uint32_t b) { return max(a, b); });
+}
+__device__ __forceinline__ float fmax_of_lanes(float v) {
+  return __uint_as_float(over_lanes(__float_as_uint(v), 0xFF800000u, [](uint32_t a, uint32_t b) {
+    return __float_as_uint(fmaxf(__uint_as_float(a), __uint_as_float(b)));
+  }));
+}
+__device__ __forceinline__ float sum_of_lanes(float v) {
+  return __uint_as_float(over_lanes(__float_as_uint(v), 0, [](uint32_t a, uint32_t b) {
+    return __float_as_uint(__uint_as_float(a) + __uint_as_float(b));
+  }));
+}
+
+// The lanes' sums against the largest entry of all.
+__device__ __forceinline__ Run join_lanes(const Run &r, float c2) {
+  const float m = fmax_of_lanes(r.m);
+  const float d = fmaxf(base_of(r.m, c2) - base_of(m, c2), -300.0f), f = exp2_fast(d);
+  return Run{m, sum_of_lanes(f * r.s), sum_of_lanes(f * __fmaf_rn(d, r.s, r.t))};
 }
 
 // What a row's results are computed from: s against the true maximum, in base e.
@@ -183,32 +214,36 @@ __device__ __forceinline__ uint64_t read_lane(uint64_t v, int lane) {
   const uint32_t hi = __builtin_amdgcn_readlane((uint32_t)(v >> 32), lane);
   return (uint64_t)hi << 32 | lo;
 }
-// the value of the lane below (DPP, a move across the whole wavefront)
-__device__ __forceinline__ uint64_t lane_below(uint64_t v) {
-  const uint32_t lo = __builtin_amdgcn_update_dpp(0u, (uint32_t)v, 0x138 /* wave_shr:1 */, 0xF, 0xF, false);
-  const uint32_t hi = __builtin_amdgcn_update_dpp(0u, (uint32_t)(v >> 32), 0x138, 0xF, 0xF, false);
-  return (uint64_t)hi << 32 | lo;
+__device__ __forceinline__ int lanes_below(uint64_t mask) {
+  return __builtin_amdgcn_mbcnt_hi((uint32_t)(mask >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)mask, 0));
 }
 
-struct BestList {
-  uint64_t mine;  // this lane's entry
-  uint64_t kth;   // the last one that counts, the same in all lanes
+// LDS written by some lanes of a wavefront and read by others of the same one: in order by itself,
+// the compiler has to keep it so.
+__device__ __forceinline__ void wave_fence() {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+}
 
-  // Put the keys of the lanes that have one better than the k-th into their places, one after
-  // the other: about 20 instructions each.
-  __device__ __forceinline__ void insert(uint64_t key, int k, int lane) {
-    uint64_t todo;
-    while ((todo = __ballot(key > kth)) != 0) {
-      const int from = __builtin_ctzll(todo);
-      const uint64_t in = read_lane(key, from);
-      const int place = __popcll(__ballot(mine > in));
-      const uint64_t below = lane_below(mine);
-      mine = lane < place ? mine : lane == place ? in : below;
-      kth = read_lane(mine, k - 1);
-      key = lane == from ? 0 : key;
-    }
+// Merge n waiting keys (in LDS) with a wavefront's list `mine`: every key's place is the number of
+// larger ones.  About 10 instructions a key that do not depend on each other; putting the
+// keys into place one after the other was 25 in one long chain.  `room`: LDS for 64 keys.
+__device__ __forceinline__ uint64_t merged_list(uint64_t mine, const uint64_t *wait, int n, uint64_t *room, int lane) {
+  wave_fence();
+  const uint64_t key = lane < n ? wait[lane] : 0;
+  int place = 0, mine_place = lane;
+  for (int i = 0; i < n; ++i) {
+    const uint64_t other = read_lane(key, i);
+    const int larger = __popcll(__ballot(mine > other));
+    place += (other > key ? 1 : 0) + (lane == i ? larger : 0);
+    mine_place += other > mine ? 1 : 0;
   }
-};
+  const int all = __popcll(__ballot(mine != 0)) + n;
+  if (mine && mine_place < 64) room[mine_place] = mine;
+  if (key && place < 64) room[place] = key;
+  wave_fence();
+  return lane < all ? room[lane] : 0;
+}
 
 // A value that at least k lanes' values reach, and the upper half of the k-th largest of them: bit
 // by bit, the largest that k lanes still reach.
@@ -235,6 +270,10 @@ __global__ void __launch_bounds__(64 * WAVES) logprobs_rows(LogprobArgs a) {
   __shared__ Run runs[WAVES];
   __shared__ uint64_t room[2][WAVES];
   __shared__ uint32_t floors[WAVES];
+  __shared__ int found;
+  __shared__ uint64_t waiting[TOP ? WAVES : 1][64], merged[TOP ? WAVES : 1][64];
+  __shared__ Pack<T, E> packed[TOP ? WAVES : 1][64];
+  __shared__ int from[TOP ? WAVES : 1][64];
   __shared__ uint64_t lists[TOP ? WAVES * TWG_LOGPROBS_MAX_TOP_K : 1], joined[TOP ? TWG_LOGPROBS_MAX_TOP_K : 1];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, k = a.top_k;
   const int64_t row = a.splits == 1 ? blockIdx.x : blockIdx.x / a.splits;
@@ -252,7 +291,8 @@ __global__ void __launch_bounds__(64 * WAVES) logprobs_rows(LogprobArgs a) {
 
   Run r{-INFINITY, 0.0f, 0.0f};
   float b = base_of(r.m, c2);
-  BestList best{0, 0};
+  uint64_t mine = 0, kth = 0;  // this lane's alternative, and the wavefront's last that counts
+  int pending = 0;             // keys in `waiting`
 
   // n values of this lane, `top` the largest, into its running sums
   auto add = [&](const float *v, float top, auto n) {
@@ -270,16 +310,46 @@ __global__ void __launch_bounds__(64 * WAVES) logprobs_rows(LogprobArgs a) {
       r.t = __fmaf_rn(e, fmaxf(d, -300.0f), r.t);
     }
   };
+  auto merge = [&]() {
+    mine = merged_list(mine, waiting[TOP ? wave : 0], pending, merged[TOP ? wave : 0], lane);
+    kth = read_lane(mine, k - 1);
+    pending = 0;
+  };
   // the few single elements at an end of the row: the first lanes of the first wavefront
-  auto edge = [&](int from, int n) {
+  auto edge = [&](int start, int n) {
     if (wave != 0 || n == 0) return;
     const bool has = lane < n;
-    const float v = has ? (float)x[from + lane] : -INFINITY;
+    const float v = has ? (float)x[start + lane] : -INFINITY;
     add(&v, v, std::integral_constant<int, 1>());
-    if (TOP) best.insert(has ? key_of(v, (uint32_t)(from + lane)) : 0, k, lane);
+    if (TOP) {
+      if (has) waiting[0][pending + lane] = key_of(v, (uint32_t)(start + lane));
+      pending += n;
+    }
+  };
+  // The bar for alternatives: candidates are above it; while `any`, -inf counts, too.
+  const int share = TOP ? (k + WAVES - 1) / WAVES : 1;
+  uint32_t floor = 0;  // a rank that at least k elements of the row reach, as far as known
+  bool any = true;
+  float bar = -INFINITY;
+  auto lowest_floor = [&]() {
+    uint32_t f = 0xFFFFFFFFu;
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w)
+      f = min(f, __hip_atomic_load(&floors[w], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP));
+    return (uint32_t)__builtin_amdgcn_readfirstlane((int)f);
+  };
+  auto raise_floor = [&]() {
+    const uint32_t at = (uint32_t)(read_lane(mine, share - 1) >> 32);
+    if (WAVES > 1 && lane == 0 && at > floors[wave])
+      __hip_atomic_store(&floors[wave], at, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+  };
+  auto set_bar = [&]() {
+    const uint32_t least = max(floor, kth ? (uint32_t)(kth >> 32) + 1 : 0u);
+    any = least <= rank_of(-INFINITY);
+    // the value one rank below (0x7FFFFFFF, which would be -0, is not in use)
+    bar = any ? -INFINITY : value_of_rank(least - (least == 0x80000000u ? 2 : 1));
   };
   // kUnroll packs of this lane, the first one pack `p` + threadIdx.x
-  uint32_t floor = 0;  // a rank that at least k elements of the row reach, as far as known
   auto step = [&](int p, auto whole) {
     Pack<T, E> raw[kUnroll];
     bool in[kUnroll];
@@ -306,46 +376,52 @@ __global__ void __launch_bounds__(64 * WAVES) logprobs_rows(LogprobArgs a) {
       // of the row reach `floor`, the smallest of the wavefronts' `floors`: in its first step
       // each knows a value that ceil(k / WAVES) of its lanes' maxima reach, later the
       // ceil(k / WAVES)-th of its list.
-      const uint32_t rank = rank_of(top);
       if (p == first) {
-        const uint32_t mine = kth_of_lanes(rank, (k + WAVES - 1) / WAVES);
-        floor = mine;
+        const uint32_t known = kth_of_lanes(rank_of(top), share);
         if (WAVES > 1) {
-          if (lane == 0) floors[wave] = mine;
+          if (lane == 0) floors[wave] = known;
           __syncthreads();
         }
+        floor = WAVES > 1 ? lowest_floor() : known;
+        set_bar();
       }
-      if (WAVES > 1) {
-        uint32_t all = 0xFFFFFFFFu;
-#pragma unroll
-        for (int w = 0; w < WAVES; ++w)
-          all = min(all, __hip_atomic_load(&floors[w], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP));
-        floor = p == first ? all : max(floor, all);
-      }
-      const uint32_t least = max(floor, best.kth ? (uint32_t)(best.kth >> 32) + 1 : 0u);
-      if (__ballot(rank >= least)) {
-        // `any`: entries of -inf count, too.  Otherwise above the value one rank below `least` (0x7FFFFFFF,
-        // which would be -0, is not in use).
-        const bool any = least <= rank_of(-INFINITY);
-        const float bar = any ? -INFINITY : value_of_rank(least - (least == 0x80000000u ? 2 : 1));
+      if (any || __ballot(top > bar)) {
+        if (WAVES > 1 && p != first) {
+          floor = max(floor, lowest_floor());
+          set_bar();
+        }
+        // The packs that hold a candidate go through LDS, so that each lane has one element of them
+        // to look at.
 #pragma unroll
         for (int u = 0; u < kUnroll; ++u) {
-          if (!any && !__ballot(most[u] > bar)) continue;
-#pragma unroll
-          for (int j = 0; j < E; ++j) {
-            const float e = v[u * E + j];
-            const bool cand = any ? in[u] : e > bar;
-            if (__ballot(cand)) {
-              const uint32_t id = (uint32_t)(head + (p + u * THREADS + (int)threadIdx.x) * E + j);
-              best.insert(cand ? key_of(e, id) : 0, k, lane);
-            }
+          const int at = p + u * THREADS + (int)threadIdx.x;
+          const uint64_t holds = __ballot(in[u] && (any || most[u] > bar));
+          if (!holds) continue;
+          if (holds >> lane & 1) {
+            const int place = lanes_below(holds);
+            packed[wave][place] = raw[u];
+            from[wave][place] = at;
           }
+          wave_fence();
+          const int n = __popcll(holds) * E;
+          for (int i = lane; i - lane < n; i += 64) {
+            const float e = i < n ? (float)((const T *)packed[wave])[i] : 0.0f;
+            const uint64_t key = i < n ? key_of(e, (uint32_t)(head + from[wave][i / E] * E + i % E)) : 0;
+            bool cand = key > kth && (any || e > bar);
+            uint64_t mask = __ballot(cand);
+            if (pending + __popcll(mask) > 64) {
+              merge();
+              cand = cand && key > kth;
+              mask = __ballot(cand);
+            }
+            if (cand) waiting[wave][pending + lanes_below(mask)] = key;
+            pending += __popcll(mask);
+          }
+          wave_fence();
         }
-        if (WAVES > 1) {
-          const uint32_t at = (uint32_t)(read_lane(best.mine, (k + WAVES - 1) / WAVES - 1) >> 32);
-          if (lane == 0 && at > floors[wave])
-            __hip_atomic_store(&floors[wave], at, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
-        }
+        merge();
+        raise_floor();
+        set_bar();
       }
     }
   };
@@ -355,32 +431,40 @@ __global__ void __launch_bounds__(64 * WAVES) logprobs_rows(LogprobArgs a) {
   for (; p + kUnroll * THREADS <= last; p += kUnroll * THREADS) step(p, std::true_type());
   if (p < last) step(p, std::false_type());
   if (split == a.splits - 1) edge(a.vocab - tail, tail);
+  if (TOP && pending) merge();
 
   // join the lanes, then the wavefronts
-#pragma unroll
-  for (int i = 1; i < 64; i <<= 1) r = join(r, shuffled(r, i), c2);
+  r = join_lanes(r, c2);
   if (WAVES > 1) {
     if (lane == 0) runs[wave] = r;
-    if (TOP && lane < k) lists[wave * k + lane] = best.mine;
-    if (TOP && (int)threadIdx.x < k) joined[threadIdx.x] = 0;
+    if (TOP) {  // of the lists only what reaches the last floor is looked at
+      if (first == last && lane == 0) floors[wave] = 0;
+      raise_floor();
+      if (threadIdx.x == 0) found = 0;
+      if ((int)threadIdx.x < k) joined[threadIdx.x] = 0;
+    }
     __syncthreads();
     r = runs[0];
 #pragma unroll
     for (int i = 1; i < WAVES; ++i) r = join(r, runs[i], c2);
     if (TOP) {  // the place of each key among all of them
-      if ((int)threadIdx.x < WAVES * k) {
+      if (lane < k && mine && (uint32_t)(mine >> 32) >= lowest_floor())
+        lists[__hip_atomic_fetch_add(&found, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP)] = mine;
+      __syncthreads();
+      const int n = found;
+      if ((int)threadIdx.x < n) {
         const uint64_t key = lists[threadIdx.x];
         int place = 0;
-        for (int i = 0; i < WAVES * k; ++i) place += lists[i] > key;
-        if (key && place < k) joined[place] = key;
+        for (int i = 0; i < n; ++i) place += lists[i] > key;
+        if (place < k) joined[place] = key;
       }
       __syncthreads();
-      best.mine = lane < k ? joined[lane] : 0;
+      mine = lane < k ? joined[lane] : 0;
     }
   }
   if (a.splits > 1) {
     const int64_t part = blockIdx.x;
-    if (TOP && (int)threadIdx.x < k) a.scratch[part * k + threadIdx.x] = best.mine;
+    if (TOP && (int)threadIdx.x < k) a.scratch[part * k + threadIdx.x] = mine;
     if (threadIdx.x == 0) {
       Run *to = (Run *)(a.scratch + a.rows * a.splits * k) + part;
       *to = r;
@@ -393,20 +477,7 @@ __global__ void __launch_bounds__(64 * WAVES) logprobs_rows(LogprobArgs a) {
   }
   const RowStats st = stats_of(r, c2);
   if (threadIdx.x == 0) put_row<T>(a, row, st);
-  if (TOP && (int)threadIdx.x < k) put_top(a, row, threadIdx.x, best.mine, st);
-}
-
-// the largest of the lanes' values, by moves within and across rows of 16 lanes (DPP)
-__device__ __forceinline__ uint32_t max_of_lanes(uint32_t v) {
-#define TWG_MAX_STEP(ctrl, rows) v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, ctrl, rows, 0xF, false))
-  TWG_MAX_STEP(0x111, 0xF);  // row_shr:1
-  TWG_MAX_STEP(0x112, 0xF);  // row_shr:2
-  TWG_MAX_STEP(0x114, 0xF);  // row_shr:4
-  TWG_MAX_STEP(0x118, 0xF);  // row_shr:8: lane 15 of each row has the row's
-  TWG_MAX_STEP(0x142, 0xA);  // row_bcast:15
-  TWG_MAX_STEP(0x143, 0xC);  // row_bcast:31: lane 63 has all
-#undef TWG_MAX_STEP
-  return (uint32_t)__builtin_amdgcn_readlane((int)v, 63);
+  if (TOP && (int)threadIdx.x < k) put_top(a, row, threadIdx.x, mine, st);
 }
 
 constexpr int kMaxSplits = 64;  // one lane each when they are joined
@@ -426,8 +497,7 @@ __global__ void __launch_bounds__(kThreads) logprobs_join(LogprobArgs a) {
     const Run *parts = (const Run *)(a.scratch + a.rows * splits * k) + row * splits;
     Run r{-INFINITY, 0.0f, 0.0f};
     if ((int)threadIdx.x < splits) r = parts[threadIdx.x];
-#pragma unroll
-    for (int i = 1; i < 64; i <<= 1) r = join(r, shuffled(r, i), c2);
+    r = join_lanes(r, c2);
     if (threadIdx.x == 0) whole = r;
   }
   __syncthreads();
@@ -558,15 +628,18 @@ LogprobArgs args_of(const twg_token_logprobs_t *d) {
 }
 
 struct RowShape {
-  int waves;   // wavefronts per workgroup
+  int waves;   // wavefronts per workgroup: 1, 4 or 8
   int splits;  // workgroups per row
 };
 
-// A row that one wavefront reads in two steps is one wavefront's; few longer rows are split so that
-// there are about 1024 workgroups, each with one step of its own at least.
+// A row that one wavefront reads in two steps is one wavefront's.  Of longer rows, 1024 and more have
+// enough work in workgroups of 4 wavefronts; fewer take 8, and fewer than 256 are split into
+// workgroups of 4 that read one step of their own at least, about 1024 in all.
 RowShape shape_of(const twg_token_logprobs_t *d) {
   const int64_t step = 16 * kUnroll / nn_size(d->dtype) * 64;  // elements a wavefront takes at a time
   if (d->vocab <= 2 * step) return RowShape{1, 1};
+  if (d->rows >= 1024) return RowShape{4, 1};
+  if (d->rows >= 256) return RowShape{8, 1};
   int64_t splits = (1024 + d->rows - 1) / d->rows;
   const int64_t steps = (d->vocab + 4 * step - 1) / (4 * step);
   splits = splits < steps ? splits : steps;
@@ -612,14 +685,16 @@ int twg_token_logprobs(const twg_token_logprobs_t *d, void *scratch, size_t scra
   return nn_dispatch(d->dtype, [&](auto t) {
     using T = decltype(t);
     const unsigned grid = (unsigned)(d->rows * shape.splits);
-    if (shape.waves == 1 && a.top_k)
-      logprobs_rows<T, 1, true><<<grid, 64, 0, s>>>(a);
-    else if (shape.waves == 1)
-      logprobs_rows<T, 1, false><<<grid, 64, 0, s>>>(a);
-    else if (a.top_k)
-      logprobs_rows<T, 4, true><<<grid, 256, 0, s>>>(a);
-    else
-      logprobs_rows<T, 4, false><<<grid, 256, 0, s>>>(a);
+    const auto go = [&](auto waves) {
+      constexpr int W = decltype(waves)::value;
+      if (a.top_k)
+        logprobs_rows<T, W, true><<<grid, 64 * W, 0, s>>>(a);
+      else
+        logprobs_rows<T, W, false><<<grid, 64 * W, 0, s>>>(a);
+    };
+    if (shape.waves == 1) go(std::integral_constant<int, 1>());
+    else if (shape.waves == 4) go(std::integral_constant<int, 4>());
+    else go(std::integral_constant<int, 8>());
     if (shape.splits > 1) logprobs_join<T><<<(unsigned)d->rows, kThreads, 0, s>>>(a);
     return (int)hipGetLastError();
   });
