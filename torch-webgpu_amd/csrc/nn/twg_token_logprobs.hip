@@ -294,6 +294,7 @@ __global__ void __launch_bounds__(64 * WAVES) logprobs_rows(LogprobArgs a) {
   uint64_t mine = 0, kth = 0;  // this lane's alternative, and the wavefront's last that counts
   int pending = 0;             // keys in `waiting`
 
+  bool masked = false;  // the same in all lanes
   // n values of this lane, `top` the largest, into its running sums
   auto add = [&](const float *v, float top, auto n) {
     if (top > r.m) {
@@ -303,9 +304,25 @@ __global__ void __launch_bounds__(64 * WAVES) logprobs_rows(LogprobArgs a) {
       r.m = top;
       b = nb;
     }
+    // An entry of -inf makes the product 0 * -inf: from the first one on the wavefront keeps
+    // its exponents finite, one instruction more for each element.
+    const Run before = r;
+    if (!masked) {
+#pragma unroll
+      for (int j = 0; j < decltype(n)::value; ++j) {
+        const float d = __fmaf_rn(v[j], c2, -b), e = exp2_fast(d);
+        r.s += e;
+        r.t = __fmaf_rn(e, d, r.t);
+      }
+      masked = __ballot(r.t != r.t) != 0;
+      if (!masked) return;
+      r = before;
+    }
+    float base = b;
+    asm("" : "+v"(base));  // computed anew: the exponents above are not kept in registers for this
 #pragma unroll
     for (int j = 0; j < decltype(n)::value; ++j) {
-      const float d = __fmaf_rn(v[j], c2, -b), e = exp2_fast(d);
+      const float d = __fmaf_rn(v[j], c2, -base), e = exp2_fast(d);
       r.s += e;
       r.t = __fmaf_rn(e, fmaxf(d, -300.0f), r.t);
     }
@@ -350,15 +367,29 @@ __global__ void __launch_bounds__(64 * WAVES) logprobs_rows(LogprobArgs a) {
     bar = any ? -INFINITY : value_of_rank(least - (least == 0x80000000u ? 2 : 1));
   };
   // kUnroll packs of this lane, the first one pack `p` + threadIdx.x
-  auto step = [&](int p, auto whole) {
-    Pack<T, E> raw[kUnroll];
-    bool in[kUnroll];
+  // A lane looks at few float32 elements per byte, so the next step's are on their way meanwhile
+  // (517 rows of 131072: 67 -> 53 us); with 16-bit elements the registers that
+  // takes cost more (4096 rows of 131072: 188 -> 192 us).
+  constexpr bool AHEAD = sizeof(T) == 4;
+  Pack<T, E> coming[kUnroll];
+  auto fetch = [&](int p, auto whole) {
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u) {
       const int at = p + u * THREADS + (int)threadIdx.x;
-      in[u] = decltype(whole)::value || at < last;
-      raw[u] = load_pack<true>(body + (in[u] ? at : last - 1));
+      coming[u] = load_pack<true>(body + (decltype(whole)::value ? at : min(at, last - 1)));
     }
+  };
+  auto step = [&](int p, auto whole) {
+    Pack<T, E> raw[kUnroll];
+    bool in[kUnroll];
+    if (!AHEAD) fetch(p, whole);
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) {
+      raw[u] = coming[u];
+      in[u] = decltype(whole)::value || p + u * THREADS + (int)threadIdx.x < last;
+    }
+    if (AHEAD && decltype(whole)::value && p + kUnroll * THREADS < last)
+      fetch(p + kUnroll * THREADS, std::false_type());
     float v[N], most[kUnroll];
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u) {
@@ -368,7 +399,9 @@ __global__ void __launch_bounds__(64 * WAVES) logprobs_rows(LogprobArgs a) {
 #pragma unroll
       for (int j = 3; j < E; j += 2) most[u] = max3(most[u], v[u * E + j], v[u * E + (j + 1 < E ? j + 1 : j)]);
     }
-    const float top = max3(max3(most[0], most[1], most[2]), most[3], most[3]);
+    float top = most[0];
+#pragma unroll
+    for (int u = 1; u < kUnroll; ++u) top = fmaxf(top, most[u]);
     add(v, top, std::integral_constant<int, N>());
     if constexpr (TOP) {
       // Which elements may be among the best k.  One of a later step has a higher id than all in
@@ -428,7 +461,10 @@ __global__ void __launch_bounds__(64 * WAVES) logprobs_rows(LogprobArgs a) {
 
   if (split == 0) edge(0, head);
   int p = first;
-  for (; p + kUnroll * THREADS <= last; p += kUnroll * THREADS) step(p, std::true_type());
+  if (AHEAD && p < last) fetch(p, std::false_type());
+  for (; p + kUnroll * THREADS <= last; p += kUnroll * THREADS) {
+    step(p, std::true_type());
+  }
   if (p < last) step(p, std::false_type());
   if (split == a.splits - 1) edge(a.vocab - tail, tail);
   if (TOP && pending) merge();
@@ -638,7 +674,7 @@ struct RowShape {
 RowShape shape_of(const twg_token_logprobs_t *d) {
   const int64_t step = 16 * kUnroll / nn_size(d->dtype) * 64;  // elements a wavefront takes at a time
   if (d->vocab <= 2 * step) return RowShape{1, 1};
-  if (d->rows >= 1024) return RowShape{4, 1};
+  if (d->rows > 512) return RowShape{4, 1};
   if (d->rows >= 256) return RowShape{8, 1};
   int64_t splits = (1024 + d->rows - 1) / d->rows;
   const int64_t steps = (d->vocab + 4 * step - 1) / (4 * step);
