@@ -194,3 +194,27 @@ def test_functions_on_tensors_want_gpu_memory():
         capi.token_logprobs(torch.zeros(2, 5), torch.zeros(2, dtype=torch.int64))
     with pytest.raises(ValueError):
         capi.dropout(torch.zeros(4), 0.5, 1)
+
+
+def test_operators_are_registered_with_their_gradients():
+    import torch_webgpu  # noqa: F401
+    for op in ("webgpu::norm_rope", "webgpu::token_logprobs", "webgpu::dropout", "aten::dropout", "aten::dropout_"):
+        lines = torch._C._dispatch_dump(op).splitlines()
+        for key in ("PrivateUse1:", "AutogradPrivateUse1:"):
+            line = [l for l in lines if l.startswith(key)]
+            assert line and "fallthrough" not in line[0], (op, key)
+
+
+def test_the_generators_state():
+    import torch_webgpu  # noqa: F401
+    before = torch.webgpu.get_rng_state()
+    torch.manual_seed(1234)
+    assert torch.webgpu.initial_seed() == 1234
+    assert not torch.equal(torch.webgpu.get_rng_state(), before)
+    torch.webgpu.set_rng_state(before)
+    assert torch.equal(torch.webgpu.get_rng_state(), before)
+    torch.webgpu.manual_seed(-1)
+    assert torch.webgpu.initial_seed() == 2 ** 64 - 1
+    with pytest.raises(ValueError):
+        torch.webgpu.set_rng_state(torch.zeros(3, dtype=torch.uint8))
+    torch.webgpu.set_rng_state(before)

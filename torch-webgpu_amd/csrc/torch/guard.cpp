@@ -2,7 +2,9 @@
 //
 // Same contract as WebGPUGuardImpl (csrc/core/webgpu_device_guard.cpp:9-49): one
 // device, a thread-local current index, the default stream only.  Adds the two
-// synchronisation hooks, which map onto the library's in-order stream.
+// synchronisation hooks, which map onto the library's in-order stream, and the backend hooks
+// that torch's autograd engine asks for (the reference registers no gradients and no hooks).
+#include <ATen/detail/PrivateUse1HooksInterface.h>
 #include <c10/core/impl/DeviceGuardImplInterface.h>
 
 #include "twg_torch.h"
@@ -50,6 +52,27 @@ struct TwgGuardImpl final : public c10::impl::DeviceGuardImplInterface {
 
   void synchronizeDevice(const c10::DeviceIndex) const override { TWG_CHECK(twg_device_sync()); }
 };
+
+struct TwgHooks final : public at::PrivateUse1HooksInterface {
+  bool isBuilt() const override { return true; }
+  bool isAvailable() const override { return twg_init() == 0; }
+  bool hasPrimaryContext(c10::DeviceIndex) const override { return twg_is_initialized() != 0; }
+  c10::DeviceIndex deviceCount() const override { return 1; }
+  c10::DeviceIndex getCurrentDevice() const override { return 0; }
+  void setCurrentDevice(c10::DeviceIndex device) const override {
+    TORCH_CHECK(device <= 0, "webgpu has a single device, got index ", (int)device);
+  }
+  c10::DeviceIndex exchangeDevice(c10::DeviceIndex device) const override {
+    setCurrentDevice(device);
+    return 0;
+  }
+  c10::DeviceIndex maybeExchangeDevice(c10::DeviceIndex) const override { return 0; }
+};
+
+const bool hooks_registered = [] {
+  at::RegisterPrivateUse1HooksInterface(new TwgHooks());  // for the life of the process
+  return true;
+}();
 
 }  // namespace
 

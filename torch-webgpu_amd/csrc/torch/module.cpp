@@ -6,6 +6,11 @@
 
 #include "twg.h"
 
+namespace torch_webgpu {
+void set_rng_state(uint64_t seed, uint64_t offset);
+void get_rng_state(uint64_t *seed, uint64_t *offset);
+}  // namespace torch_webgpu
+
 namespace {
 
 PyObject *raise_twg(int rc) {
@@ -54,6 +59,19 @@ PyObject *py_device_info(PyObject *, PyObject *) {
                        (long long)mem);
 }
 
+PyObject *py_set_rng_state(PyObject *, PyObject *args) {
+  unsigned long long seed = 0, offset = 0;
+  if (!PyArg_ParseTuple(args, "KK", &seed, &offset)) return nullptr;
+  torch_webgpu::set_rng_state(seed, offset);
+  Py_RETURN_NONE;
+}
+
+PyObject *py_get_rng_state(PyObject *, PyObject *) {
+  uint64_t seed = 0, offset = 0;
+  torch_webgpu::get_rng_state(&seed, &offset);
+  return Py_BuildValue("KK", (unsigned long long)seed, (unsigned long long)offset);
+}
+
 PyMethodDef methods[] = {
     {"_init", py_init, METH_NOARGS, "Bind the GPU and create the stream."},
     {"_is_initialized", py_is_initialized, METH_NOARGS, "True once the GPU is bound."},
@@ -61,6 +79,8 @@ PyMethodDef methods[] = {
     {"_empty_cache", py_empty_cache, METH_NOARGS, "Return cached device blocks to the driver."},
     {"_memory_stats", py_memory_stats, METH_NOARGS, "Allocator counters."},
     {"_device_info", py_device_info, METH_NOARGS, "Name, compute units and memory of the GPU."},
+    {"_set_rng_state", py_set_rng_state, METH_VARARGS, "Seed of dropout's generator and offset of its next call."},
+    {"_get_rng_state", py_get_rng_state, METH_NOARGS, "(seed, offset) of dropout's generator."},
     {nullptr, nullptr, 0, nullptr}};
 
 struct PyModuleDef module_def = {PyModuleDef_HEAD_INIT, "torch_webgpu._C",

@@ -55,4 +55,8 @@ void fill_iter(const at::TensorIteratorBase &iter, twg_iter_t *out);
 // logical dimension fastest (row-major walk), for ops whose element order matters.
 void fill_iter_logical(const at::Tensor &a, const at::Tensor &b, twg_iter_t *out);
 
+// The generator behind dropout on the device: the seed, and the offset of the next call.
+void set_rng_state(uint64_t seed, uint64_t offset);
+void get_rng_state(uint64_t *seed, uint64_t *offset);
+
 }  // namespace torch_webgpu

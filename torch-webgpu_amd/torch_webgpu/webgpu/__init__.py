@@ -5,12 +5,16 @@
 device plumbing (seeding, `torch.get_device_module`) and users of a real GPU
 backend look for.
 """
+import struct
+
+import torch
+
 from .. import _C
 
 __all__ = [
     "is_initialized", "current_device", "device_count", "is_available", "init", "synchronize",
     "empty_cache", "memory_stats", "get_device_name", "get_device_properties", "manual_seed_all",
-    "manual_seed",
+    "manual_seed", "initial_seed", "get_rng_state", "set_rng_state",
 ]
 
 
@@ -61,15 +65,32 @@ def get_device_name(device=None):
     return _C._device_info()["name"]
 
 
-# No op on this path draws random numbers; these exist so that torch.manual_seed()
-# does not warn about a backend without seeding hooks.
+# What draws random numbers on the device is dropout.  Its generator is counter-based: a seed, and
+# an offset that every call takes one of; torch.manual_seed() sets it through these hooks.
 def _is_in_bad_fork():
     return False
 
 
 def manual_seed_all(seed):
-    return None
+    """Seed dropout's generator and start its offsets at 0 (torch.manual_seed() does this)."""
+    _C._set_rng_state(int(seed) & (2 ** 64 - 1), 0)
 
 
 def manual_seed(seed):
-    return None
+    manual_seed_all(seed)
+
+
+def initial_seed():
+    return _C._get_rng_state()[0]
+
+
+def get_rng_state(device=None):
+    """The generator's seed and next offset as 16 bytes."""
+    return torch.tensor(list(struct.pack("<QQ", *_C._get_rng_state())), dtype=torch.uint8)
+
+
+def set_rng_state(new_state, device=None):
+    """Put the generator back to what get_rng_state returned."""
+    if new_state.dtype != torch.uint8 or new_state.numel() != 16:
+        raise ValueError("expected the 16 bytes that get_rng_state returns")
+    _C._set_rng_state(*struct.unpack("<QQ", bytes(new_state.tolist())))
