@@ -138,6 +138,56 @@ __global__ void __launch_bounds__(kDenseThreads) dropout_packs(T *out, const T *
   }
 }
 
+// The same for dense float32, where a group is two packs: lane by lane, a wavefront's loads and
+// stores would each touch every other 16 bytes.  The lanes take packs side by side
+// instead, 64 and the next 64, and find the words of a pack's group in LDS, where lane g has put those of
+// group g.
+template <bool RES, bool STREAM>
+__global__ void __launch_bounds__(64) dropout_pairs(float *out, const float *x, const float *res, int64_t numel, DropArgs a) {
+  typedef Pack<float, 4> Vec;
+  __shared__ Pack<uint32_t, 4> words[64];
+  const int lane = threadIdx.x;
+  const int64_t e0 = (int64_t)blockIdx.x * 64 * kPer;
+  Vec vx[2], vr[2];
+#pragma unroll
+  for (int u = 0; u < 2; ++u) {
+    const int64_t e = e0 + (u * 64 + lane) * 4;
+    if (e + 4 <= numel) {
+      vx[u] = load_pack<STREAM>(reinterpret_cast<const Vec *>(x + e));
+      if (RES) vr[u] = load_pack<STREAM>(reinterpret_cast<const Vec *>(res + e));
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if (e + j >= numel) continue;
+        vx[u].v[j] = x[e + j];
+        if (RES) vr[u].v[j] = res[e + j];
+      }
+    }
+  }
+  const Words w = philox((uint64_t)(e0 / kPer + lane), total_offset(a), a.seed);
+  words[lane] = Pack<uint32_t, 4>{{w.w[0], w.w[1], w.w[2], w.w[3]}};
+  __syncthreads();
+#pragma unroll
+  for (int u = 0; u < 2; ++u) {
+    const int64_t e = e0 + (u * 64 + lane) * 4;
+    const uint32_t *half = &words[u * 32 + lane / 2].v[2 * (lane & 1)];
+    const uint32_t h0 = half[0], h1 = half[1];
+    Vec o;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const uint32_t bits = ((j < 2 ? h0 : h1) >> (16 * (j & 1))) & 0xFFFFu;
+      o.v[j] = dropped(vx[u].v[j], RES ? vr[u].v[j] : 0.0f, bits, a);
+    }
+    if (e + 4 <= numel) {
+      store_pack<STREAM>(reinterpret_cast<Vec *>(out + e), o);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (e + j < numel) out[e + j] = o.v[j];
+    }
+  }
+}
+
 // Whether every operand's groups of 8 elements are two or one aligned packs.
 bool packs_fit(const Geom &g, const void *out, const void *x, const void *res, int size) {
   if (!aligned_to(out, 16) || !aligned_to(x, 16) || !aligned_to(res, 16)) return false;
@@ -158,16 +208,28 @@ int launch_dropout(T *out, const T *x, const T *res, const Geom &g, const DropAr
     const int64_t small = (groups + kDenseThreads - 1) / kDenseThreads;
     if (small > INT32_MAX) return TWG_E_TOO_LARGE;
     const bool stream = g.numel * (int64_t)sizeof(T) * (res ? 3 : 2) > kStreamBytes, dense = g.ndim <= 1;
+    if constexpr (sizeof(T) == 4) {
+      if (dense) {
+        if (res && stream) dropout_pairs<true, true><<<(unsigned)small, 64, 0, s>>>(out, x, res, g.numel, a);
+        else if (res) dropout_pairs<true, false><<<(unsigned)small, 64, 0, s>>>(out, x, res, g.numel, a);
+        else if (stream) dropout_pairs<false, true><<<(unsigned)small, 64, 0, s>>>(out, x, res, g.numel, a);
+        else dropout_pairs<false, false><<<(unsigned)small, 64, 0, s>>>(out, x, res, g.numel, a);
+        return (int)hipGetLastError();
+      }
+    }
 #define TWG_DROP(RES, DENSE, STREAM) \
   dropout_packs<T, RES, DENSE, STREAM><<<(unsigned)small, kDenseThreads, 0, s>>>(out, x, res, g, a)
-    if (res && dense && stream) TWG_DROP(true, true, true);
-    else if (res && dense) TWG_DROP(true, true, false);
-    else if (res && stream) TWG_DROP(true, false, true);
-    else if (res) TWG_DROP(true, false, false);
-    else if (dense && stream) TWG_DROP(false, true, true);
-    else if (dense) TWG_DROP(false, true, false);
-    else if (stream) TWG_DROP(false, false, true);
-    else TWG_DROP(false, false, false);
+    if (sizeof(T) == 2 && dense) {
+      if (res && stream) TWG_DROP(true, sizeof(T) == 2, true);
+      else if (res) TWG_DROP(true, sizeof(T) == 2, false);
+      else if (stream) TWG_DROP(false, sizeof(T) == 2, true);
+      else TWG_DROP(false, sizeof(T) == 2, false);
+    } else {
+      if (res && stream) TWG_DROP(true, false, true);
+      else if (res) TWG_DROP(true, false, false);
+      else if (stream) TWG_DROP(false, false, true);
+      else TWG_DROP(false, false, false);
+    }
 #undef TWG_DROP
     return (int)hipGetLastError();
   }

@@ -567,7 +567,9 @@ template <typename T, bool STREAM>
 __global__ void __launch_bounds__(kThreads) logprobs_grad(LogprobArgs a) {
   constexpr int E = 16 / (int)sizeof(T), PER = kGradPacks * kThreads;
   typedef Pack<T, E> Vec;
-  const int64_t row = blockIdx.x;
+  const uint32_t chunks = (uint32_t)a.splits;  // workgroups of a row, one behind the other in memory
+  const int64_t row = blockIdx.x / chunks;
+  const int first_chunk = (int)(blockIdx.x - (uint32_t)row * chunks);
   const T *x = (const T *)a.logits + row * a.row_stride;
   T *grad = (T *)a.grad + row * a.grad_stride;
   const int64_t t = target_of(a, row);
@@ -592,7 +594,7 @@ __global__ void __launch_bounds__(kThreads) logprobs_grad(LogprobArgs a) {
   const int head = lead < a.vocab ? lead : a.vocab;
   const int packs = (a.vocab - head) / E, tail = a.vocab - head - packs * E;
   const bool alike = (((uintptr_t)x ^ (uintptr_t)grad) & 15) == 0;  // the logits' packs are aligned, too
-  for (int chunk = blockIdx.y; chunk * PER < packs || chunk == 0; chunk += gridDim.y) {
+  for (int chunk = first_chunk; chunk * PER < packs || chunk == 0; chunk += chunks) {
     if (chunk == 0 && (int)threadIdx.x < head + tail) {
       const int j = (int)threadIdx.x < head ? threadIdx.x : a.vocab - tail + (int)threadIdx.x - head;
       grad[j] = (T)(none ? 0.0f : one((float)x[j], j));
@@ -750,8 +752,10 @@ int twg_token_logprobs_backward(const twg_token_logprobs_t *d, twg_stream_t stre
   a.grad_stride = d->grad_stride;
   return nn_dispatch(d->dtype, [&](auto t) {
     using T = decltype(t);
-    const int64_t per = kGradPacks * kThreads * 16 / (int)sizeof(T), chunks = (d->vocab + per - 1) / per;
-    const dim3 grid((unsigned)d->rows, (unsigned)(chunks < 65535 ? chunks : 65535));
+    const int64_t per = kGradPacks * kThreads * 16 / (int)sizeof(T), most = INT32_MAX / d->rows;
+    const int64_t chunks = (d->vocab + per - 1) / per;
+    a.splits = (int32_t)(chunks < most ? chunks : most);
+    const unsigned grid = (unsigned)(d->rows * a.splits);
     if (2.0 * (double)d->rows * (double)d->vocab * sizeof(T) > (double)kStreamBytes)
       logprobs_grad<T, true><<<grid, kThreads, 0, nn_stream(stream)>>>(a);
     else
