@@ -15,6 +15,7 @@ namespace {
 constexpr int kMaxPairs = TWG_ROPE_MAX_HEAD_DIM / 2;
 constexpr int kTrigRoom = 1024;  // cosines (and sines) a workgroup holds: 8 KiB of LDS
 constexpr int kMaxTile = 16;     // tokens a workgroup takes at most
+constexpr int kSteps = 4;        // heads a group takes in a piece of work where there are many
 
 // Queries and keys are two parts, each with workgroups of its own: what differs between the parts
 // is the same for a whole workgroup.
@@ -34,7 +35,7 @@ struct RopeArgs {
   int32_t pairs, rot_pairs;  // head_dim / 2, rot_dim / 2
   int32_t log_g;             // log2 of the lanes per head
   int32_t position_dtype;
-  int32_t norm;
+  int32_t norm, n_axes;
   float eps, inv_dim;
   uint32_t all_tokens, tokens;  // batch * tokens, tokens of one sequence
   int64_t pos_stride[3];
@@ -63,15 +64,38 @@ __device__ __forceinline__ void turn(double pos, float inv_freq, float *c, float
   sincospif(half_turns, s, c);
 }
 
-// What a lane holds of one head: V pairs as two runs of V elements of memory.  `first` is
-// where the run of the first elements starts, `second` the other.  Pairs beyond the rotated
-// ones are neighbours.
+// What a lane holds of chunk c of a head: V pairs as two runs of V elements of memory, and where
+// their cosines are.  With pairs in halves the runs hold the pairs' first and second members; beyond the
+// rotated elements they are neighbours.  With adjacent pairs a run is V / 2 whole pairs, and the lanes'
+// runs lie side by side, so that every load is of whole lines.
 template <int V, bool ADJ>
-__device__ __forceinline__ void runs_of(const RopeArgs &a, int p0, int *first, int *second) {
-  const bool halves = !ADJ && p0 < a.rot_pairs;
-  *first = halves ? p0 : 2 * p0;
-  *second = halves ? p0 + a.rot_pairs : 2 * p0 + V;
-}
+struct Runs {
+  static constexpr bool kWhole = ADJ && V > 1;  // runs of whole pairs
+  int first, second;                            // element offsets in the head
+  bool has0, has1;                              // inside the head
+  bool rot0, rot1;                              // rotated
+  int trig0, trig1;                             // pair numbers
+  __device__ __forceinline__ Runs(int pairs, int rot_pairs, int log_g, int c, int lane) {
+    if constexpr (kWhole) {
+      first = (((2 * c) << log_g) + lane) * V;
+      second = (((2 * c + 1) << log_g) + lane) * V;
+      has0 = first < 2 * pairs;
+      has1 = second < 2 * pairs;
+      rot0 = first < 2 * rot_pairs;
+      rot1 = second < 2 * rot_pairs;
+      trig0 = first / 2;
+      trig1 = second / 2;
+    } else {
+      const int p0 = ((c << log_g) + lane) * V;
+      const bool halves = !ADJ && p0 < rot_pairs;
+      first = halves ? p0 : 2 * p0;
+      second = halves ? p0 + rot_pairs : 2 * p0 + V;
+      has0 = has1 = p0 < pairs;
+      rot0 = rot1 = p0 < rot_pairs;
+      trig0 = trig1 = p0;
+    }
+  }
+};
 
 template <typename T, int V>
 __device__ __forceinline__ void load_run(float *to, const T *from) {
@@ -85,29 +109,33 @@ __device__ __forceinline__ void load_run(float *to, const T *from) {
 #pragma unroll
   for (int v = 0; v < N; ++v) to[v] = (float)p.v[v];
 }
-template <typename T, int V>
+template <bool NT, typename T, int V>
 __device__ __forceinline__ void store_run(T *to, const float *from) {
   Pack<T, V> p;
 #pragma unroll
   for (int v = 0; v < V; ++v) p.v[v] = (T)from[v];
-  store_pack<false>(reinterpret_cast<Pack<T, V> *>(to), p);
+  store_pack<NT>(reinterpret_cast<Pack<T, V> *>(to), p);
 }
 
-// Index in the lane's 2V elements (two runs, one after the other) of pair v's members.
+__device__ __forceinline__ void turn_pair(float &lo, float &hi, float c, float s) {
+  const float l = lo, h = hi;
+  lo = __fmaf_rn(l, c, -(h * s));
+  hi = __fmaf_rn(h, c, l * s);
+}
+// z: the two runs, one after the other; sign = 1 turns forward, -1 back
 template <int V, bool ADJ>
-__device__ __forceinline__ constexpr int lo_of(int v) { return ADJ ? 2 * v : v; }
-template <int V, bool ADJ>
-__device__ __forceinline__ constexpr int hi_of(int v) { return ADJ ? 2 * v + 1 : V + v; }
-
-// sign = 1 turns forward, -1 back
-template <int V, bool ADJ>
-__device__ __forceinline__ void rotate(float *z, const float *cs, const float *sn, float sign) {
+__device__ __forceinline__ void rotate(float *z, const Runs<V, ADJ> &at, const float *cs, const float *sn, float sign) {
+  if constexpr (Runs<V, ADJ>::kWhole) {
 #pragma unroll
-  for (int v = 0; v < V; ++v) {
-    float &lo = z[lo_of<V, ADJ>(v)], &hi = z[hi_of<V, ADJ>(v)];
-    const float c = cs[v], s = sign * sn[v], l = lo, h = hi;
-    lo = __fmaf_rn(l, c, -(h * s));
-    hi = __fmaf_rn(h, c, l * s);
+    for (int r = 0; r < 2; ++r) {
+      if (!(r ? at.rot1 : at.rot0)) continue;
+      const int t = r ? at.trig1 : at.trig0;
+#pragma unroll
+      for (int v = 0; v < V / 2; ++v) turn_pair(z[r * V + 2 * v], z[r * V + 2 * v + 1], cs[t + v], sign * sn[t + v]);
+    }
+  } else if (at.rot0) {
+#pragma unroll
+    for (int v = 0; v < V; ++v) turn_pair(z[v], z[V + v], cs[at.trig0 + v], sign * sn[at.trig0 + v]);
   }
 }
 
@@ -132,20 +160,22 @@ struct TokenRoom {
   int64_t x[kMaxTile], dy[kMaxTile], out[kMaxTile];
 };
 
-__device__ __forceinline__ void fill(const RopeArgs &a, const PartArgs &part, uint32_t t0, int n, TokenRoom &room) {
-  for (int i = threadIdx.x; i < n * a.rot_pairs; i += kThreads) {
-    const uint32_t lt = (uint32_t)i / (uint32_t)a.rot_pairs, p = i - lt * a.rot_pairs;
-    const uint32_t b = (t0 + lt) / a.tokens, t = t0 + lt - b * a.tokens;
-    float c, s;
-    turn(position_at(a, a.pair_axis[p], b, t), a.inv_freq[p], &c, &s);
-    room.cs[i] = c;
-    room.sn[i] = s;
-  }
+__device__ __forceinline__ void fill_offsets(const RopeArgs &a, const PartArgs &part, uint32_t t0, int n, TokenRoom &room) {
   if ((int)threadIdx.x < n) {
     const uint32_t b = (t0 + threadIdx.x) / a.tokens, t = t0 + threadIdx.x - b * a.tokens;
     room.x[threadIdx.x] = b * part.xs[0] + t * part.xs[1];
     room.dy[threadIdx.x] = b * part.ys[0] + t * part.ys[1];
     room.out[threadIdx.x] = b * part.os[0] + t * part.os[1];
+  }
+}
+__device__ __forceinline__ void fill_trig(const RopeArgs &a, uint32_t t0, int n, TokenRoom &room) {
+  for (int i = threadIdx.x; i < n * a.rot_pairs; i += kThreads) {
+    const uint32_t lt = (uint32_t)i / (uint32_t)a.rot_pairs, p = i - lt * a.rot_pairs;
+    const uint32_t b = (t0 + lt) / a.tokens, t = t0 + lt - b * a.tokens;
+    float c, s;
+    turn(position_at(a, a.n_axes == 1 ? 0 : a.pair_axis[p], b, t), a.inv_freq[p], &c, &s);
+    room.cs[i] = c;
+    room.sn[i] = s;
   }
 }
 
@@ -181,19 +211,22 @@ struct Raw {
   Pack<T, V> v[C][2];
 };
 
-template <typename T, int V, int C, bool ADJ>
+template <bool NT, typename T, int V, int C, bool ADJ>
 __device__ __forceinline__ void fetch(const RopeArgs &a, const void *base, int64_t offset, int lane, Raw<T, V, C> &to) {
   const T *from = (const T *)base + offset;
 #pragma unroll
   for (int c = 0; c < C; ++c) {
-    const int p0 = ((c << a.log_g) + lane) * V;
-    if (p0 < a.pairs) {
-      int first, second;
-      runs_of<V, ADJ>(a, p0, &first, &second);
-      to.v[c][0] = load_pack<false>((const Pack<T, V> *)(from + first));
-      to.v[c][1] = load_pack<false>((const Pack<T, V> *)(from + second));
-    }
+    const Runs<V, ADJ> at(a.pairs, a.rot_pairs, a.log_g, c, lane);
+    if (at.has0) to.v[c][0] = load_pack<NT>((const Pack<T, V> *)(from + at.first));
+    if (at.has1) to.v[c][1] = load_pack<NT>((const Pack<T, V> *)(from + at.second));
   }
+}
+
+// The runs as binary32; zeros outside the head.
+template <typename T, int V>
+__device__ __forceinline__ void widen_runs(const Pack<T, V> *raw, bool has0, bool has1, float *z) {
+#pragma unroll
+  for (int j = 0; j < 2 * V; ++j) z[j] = (j < V ? has0 : has1) ? (float)raw[j / V].v[j % V] : 0.0f;
 }
 
 // The lane's elements of a norm weight; ones without it.
@@ -202,74 +235,69 @@ __device__ __forceinline__ void fetch_weight(const RopeArgs &a, const PartArgs &
   const TW *from = (const TW *)part.weight;
 #pragma unroll
   for (int c = 0; c < C; ++c) {
-    const int p0 = ((c << a.log_g) + lane) * V;
+    const Runs<V, ADJ> at(a.pairs, a.rot_pairs, a.log_g, c, lane);
 #pragma unroll
     for (int j = 0; j < 2 * V; ++j) w[c][j] = 1.0f;
-    if (from && p0 < a.pairs) {
-      int first, second;
-      runs_of<V, ADJ>(a, p0, &first, &second);
-      load_run<TW, V>(w[c], from + first);
-      load_run<TW, V>(w[c] + V, from + second);
-    }
+    if (from && at.has0) load_run<TW, V>(w[c], from + at.first);
+    if (from && at.has1) load_run<TW, V>(w[c] + V, from + at.second);
   }
 }
 
 // A group of 2^log_g lanes works on one head at a time, a lane on V pairs in each of C chunks of
-// it.  The group's next head is on its way meanwhile.
-template <typename T, typename TW, int V, int C, bool ADJ>
+// it.  The group's next head is on its way meanwhile, the first one while the angles are computed.
+// (All of a piece's heads asked for at once: 104 registers instead of 76, 17.8 -> 21.6 us
+// for 4096 tokens x 40 heads of 128.)
+template <typename T, typename TW, int V, int C, bool ADJ, bool STREAM>
 __global__ void __launch_bounds__(kThreads) rope_forward(RopeArgs a) {
   __shared__ TokenRoom room;
   const bool second_part = (int)blockIdx.x >= a.part[0].grid;
   const PartArgs &part = a.part[second_part];
   const int lane = threadIdx.x & ((1 << a.log_g) - 1);
   Piece at(a, part, (int)blockIdx.x - (second_part ? a.part[0].grid : 0));
-  fill(a, part, at.t0, at.n, room);
-  float w[C][2 * V];
-  if (a.norm) fetch_weight<TW, V, C, ADJ>(a, part, lane, w);
+  fill_offsets(a, part, at.t0, at.n, room);
   __syncthreads();
   Raw<T, V, C> coming;
-  if (at.more()) fetch<T, V, C, ADJ>(a, part.x, room.x[at.lt] + at.h * part.xs[2], lane, coming);
+  if (at.more()) fetch<STREAM, T, V, C, ADJ>(a, part.x, room.x[at.lt] + at.h * part.xs[2], lane, coming);
+  float w[C][2 * V];
+  if (a.norm) fetch_weight<TW, V, C, ADJ>(a, part, lane, w);
+  fill_trig(a, at.t0, at.n, room);
+  __syncthreads();
   while (at.more()) {
     const Raw<T, V, C> x = coming;
     const int lt = at.lt;
     T *out = (T *)part.out + room.out[lt] + at.h * part.os[2];
     at.next();
-    if (at.more()) fetch<T, V, C, ADJ>(a, part.x, room.x[at.lt] + at.h * part.xs[2], lane, coming);
+    if (at.more()) fetch<STREAM, T, V, C, ADJ>(a, part.x, room.x[at.lt] + at.h * part.xs[2], lane, coming);
     float z[C][2 * V];
     float sq = 0.0f;
 #pragma unroll
     for (int c = 0; c < C; ++c) {
-      if (((c << a.log_g) + lane) * V >= a.pairs) continue;
+      const Runs<V, ADJ> run(a.pairs, a.rot_pairs, a.log_g, c, lane);
+      widen_runs<T, V>(x.v[c], run.has0, run.has1, z[c]);
 #pragma unroll
-      for (int j = 0; j < 2 * V; ++j) {
-        z[c][j] = (float)x.v[c][j / V].v[j % V];
-        sq = __fmaf_rn(z[c][j], z[c][j], sq);
-      }
+      for (int j = 0; j < 2 * V; ++j) sq = __fmaf_rn(z[c][j], z[c][j], sq);
     }
     float r = 1.0f;
     if (a.norm) r = 1.0f / sqrtf(__fmaf_rn(group_sum(sq, a.log_g), a.inv_dim, a.eps));
 #pragma unroll
     for (int c = 0; c < C; ++c) {
-      const int p0 = ((c << a.log_g) + lane) * V;
-      if (p0 >= a.pairs) continue;
-      int first, second;
-      runs_of<V, ADJ>(a, p0, &first, &second);
+      const Runs<V, ADJ> run(a.pairs, a.rot_pairs, a.log_g, c, lane);
       if (a.norm) {
 #pragma unroll
         for (int j = 0; j < 2 * V; ++j) z[c][j] = z[c][j] * r * w[c][j];
       }
-      if (p0 < a.rot_pairs)
-        rotate<V, ADJ>(z[c], room.cs + lt * a.rot_pairs + p0, room.sn + lt * a.rot_pairs + p0, 1.0f);
-      store_run<T, V>(out + first, z[c]);
-      store_run<T, V>(out + second, z[c] + V);
+      rotate<V, ADJ>(z[c], run, room.cs + lt * a.rot_pairs, room.sn + lt * a.rot_pairs, 1.0f);
+      if (run.has0) store_run<STREAM, T, V>(out + run.first, z[c]);
+      if (run.has1) store_run<STREAM, T, V>(out + run.second, z[c] + V);
     }
   }
 }
 
-// The same walk, over as many pieces as there are for the workgroup: its sums of dz u for the
-// weight's gradient stay in registers until the last one is done.
-template <typename T, typename TW, int V, int C, bool ADJ>
-__global__ void __launch_bounds__(kThreads) rope_backward(RopeArgs a) {
+// The same walk, over as many pieces as there are for the workgroup, the group's next head on its way
+// while it works on one: its sums of dz u for the weight's gradient stay in registers until the last
+// piece is done.
+template <typename T, typename TW, int V, int C, bool ADJ, bool STREAM>
+__global__ void __launch_bounds__(kThreads, 4) rope_backward(RopeArgs a) {
   __shared__ TokenRoom room;
   __shared__ float joined[2 * kMaxPairs];
   const bool second_part = (int)blockIdx.x >= a.part[0].grid;
@@ -285,14 +313,16 @@ __global__ void __launch_bounds__(kThreads) rope_backward(RopeArgs a) {
   for (int64_t piece = block; piece < part.work; piece += part.grid) {
     Piece at(a, part, (int)piece);
     __syncthreads();
-    fill(a, part, at.t0, at.n, room);
+    fill_offsets(a, part, at.t0, at.n, room);
     __syncthreads();
     Raw<T, V, C> coming_x, coming_y;
     auto get = [&]() {
-      fetch<T, V, C, ADJ>(a, part.dy, room.dy[at.lt] + at.h * part.ys[2], lane, coming_y);
-      if (a.norm) fetch<T, V, C, ADJ>(a, part.x, room.x[at.lt] + at.h * part.xs[2], lane, coming_x);
+      fetch<STREAM, T, V, C, ADJ>(a, part.dy, room.dy[at.lt] + at.h * part.ys[2], lane, coming_y);
+      if (a.norm) fetch<STREAM, T, V, C, ADJ>(a, part.x, room.x[at.lt] + at.h * part.xs[2], lane, coming_x);
     };
     if (at.more()) get();
+    fill_trig(a, at.t0, at.n, room);
+    __syncthreads();
     while (at.more()) {
       const Raw<T, V, C> x = coming_x, y = coming_y;
       const int lt = at.lt;
@@ -303,18 +333,13 @@ __global__ void __launch_bounds__(kThreads) rope_backward(RopeArgs a) {
       float sq = 0.0f, dot = 0.0f;
 #pragma unroll
       for (int c = 0; c < C; ++c) {
-        const int p0 = ((c << a.log_g) + lane) * V;
-        if (p0 >= a.pairs) continue;
-#pragma unroll
-        for (int j = 0; j < 2 * V; ++j) g[c][j] = (float)y.v[c][j / V].v[j % V];
-        if (p0 < a.rot_pairs)
-          rotate<V, ADJ>(g[c], room.cs + lt * a.rot_pairs + p0, room.sn + lt * a.rot_pairs + p0, -1.0f);
+        const Runs<V, ADJ> run(a.pairs, a.rot_pairs, a.log_g, c, lane);
+        widen_runs<T, V>(y.v[c], run.has0, run.has1, g[c]);
+        rotate<V, ADJ>(g[c], run, room.cs + lt * a.rot_pairs, room.sn + lt * a.rot_pairs, -1.0f);
         if (a.norm) {
+          widen_runs<T, V>(x.v[c], run.has0, run.has1, z[c]);
 #pragma unroll
-          for (int j = 0; j < 2 * V; ++j) {
-            z[c][j] = (float)x.v[c][j / V].v[j % V];
-            sq = __fmaf_rn(z[c][j], z[c][j], sq);
-          }
+          for (int j = 0; j < 2 * V; ++j) sq = __fmaf_rn(z[c][j], z[c][j], sq);
         }
       }
       float r = 1.0f;
@@ -322,7 +347,6 @@ __global__ void __launch_bounds__(kThreads) rope_backward(RopeArgs a) {
         r = 1.0f / sqrtf(__fmaf_rn(group_sum(sq, a.log_g), a.inv_dim, a.eps));
 #pragma unroll
         for (int c = 0; c < C; ++c) {
-          if (((c << a.log_g) + lane) * V >= a.pairs) continue;
 #pragma unroll
           for (int j = 0; j < 2 * V; ++j) {
             z[c][j] *= r;
@@ -335,16 +359,13 @@ __global__ void __launch_bounds__(kThreads) rope_backward(RopeArgs a) {
       }
 #pragma unroll
       for (int c = 0; c < C; ++c) {
-        const int p0 = ((c << a.log_g) + lane) * V;
-        if (p0 >= a.pairs) continue;
-        int first, second;
-        runs_of<V, ADJ>(a, p0, &first, &second);
+        const Runs<V, ADJ> run(a.pairs, a.rot_pairs, a.log_g, c, lane);
         if (a.norm) {
 #pragma unroll
           for (int j = 0; j < 2 * V; ++j) g[c][j] = r * __fmaf_rn(-z[c][j], dot, g[c][j]);
         }
-        store_run<T, V>(out + first, g[c]);
-        store_run<T, V>(out + second, g[c] + V);
+        if (run.has0) store_run<STREAM, T, V>(out + run.first, g[c]);
+        if (run.has1) store_run<STREAM, T, V>(out + run.second, g[c] + V);
       }
     }
   }
@@ -359,15 +380,12 @@ __global__ void __launch_bounds__(kThreads) rope_backward(RopeArgs a) {
     if ((int)(threadIdx.x >> 6) == wave && (int)(threadIdx.x & 63) < (1 << a.log_g)) {
 #pragma unroll
       for (int c = 0; c < C; ++c) {
-        const int p0 = ((c << a.log_g) + lane) * V;
-        if (p0 < a.pairs) {
-          int first, second;
-          runs_of<V, ADJ>(a, p0, &first, &second);
+        const Runs<V, ADJ> run(a.pairs, a.rot_pairs, a.log_g, c, lane);
 #pragma unroll
-          for (int j = 0; j < 2 * V; ++j) {
-            float &to = joined[j < V ? first + j : second + j - V];
-            to = wave ? to + dw[c][j] : dw[c][j];
-          }
+        for (int j = 0; j < 2 * V; ++j) {
+          if (!(j < V ? run.has0 : run.has1)) continue;
+          float &to = joined[j < V ? run.first + j : run.second + j - V];
+          to = wave ? to + dw[c][j] : dw[c][j];
         }
       }
     }
@@ -459,7 +477,8 @@ int check(const twg_norm_rope_t *d, bool backward) {
 
 // Whether every run of v elements that a lane moves is aligned to its own size.
 bool runs_aligned(const twg_norm_rope_t *d, bool backward, int v) {
-  if ((d->head_dim / 2) % v || (d->rot_dim / 2) % v) return false;
+  const int whole = d->adjacent && v > 1 ? 2 : 1;  // pairs in a run's elements
+  if ((d->head_dim * whole / 2) % v || (d->rot_dim * whole / 2) % v) return false;
   const size_t bytes = (size_t)(v * nn_size(d->dtype));
   const size_t wbytes = (size_t)(v * nn_size(d->weight_dtype) > 16 ? 16 : v * nn_size(d->weight_dtype));
   for (const twg_rope_part_t &p : d->part) {
@@ -484,11 +503,12 @@ Lanes lanes_of(const twg_norm_rope_t *d, bool backward) {
   return l;
 }
 
-constexpr int kMaxSums = 1536;  // workgroups of one part that leave sums for the weight's gradient
-constexpr int kSteps = 4;       // heads a group takes in a piece of work where there are many
-
-// How a part is cut into pieces: as many tokens as give each group kSteps heads (one where there is
-// too little work to fill the chip with), or a share of one token's heads.
+// Workgroups that leave sums for the weights' gradients, for both parts together at most, each with the
+// same number of pieces.  (1016, all that the chip holds at a time: 121 us instead of 117
+// for the backward call of 16384 tokens x 40 heads of 128; 8192: 113 instead of 108 with the hint below.)
+constexpr int kMaxSums = 4096;
+// How a part is cut into pieces: as many tokens as give each group kSteps heads (fewer where there
+// is too little work to fill the chip with), or a share of one token's heads.
 void cut(const twg_norm_rope_t *d, bool backward, int k, PartArgs &p) {
   const int64_t all = d->batch * d->tokens, heads = d->part[k].heads;
   p.heads = (int32_t)heads;
@@ -499,7 +519,7 @@ void cut(const twg_norm_rope_t *d, bool backward, int k, PartArgs &p) {
   const int64_t passes = all * total_heads(d) / groups / 1024;
   const int64_t want = groups * (passes < 1 ? 1 : passes < kSteps ? passes : kSteps);
   const int rot = d->rot_dim > 2 ? d->rot_dim / 2 : 1;
-  int64_t tile = (want + heads - 1) / heads;
+  int64_t tile = want / heads > 0 ? want / heads : 1;
   if (tile > kMaxTile) tile = kMaxTile;
   if (tile > kTrigRoom / rot) tile = kTrigRoom / rot;
   if (tile > all) tile = all;
@@ -509,23 +529,35 @@ void cut(const twg_norm_rope_t *d, bool backward, int k, PartArgs &p) {
   p.split = (int32_t)(tiles * split > INT32_MAX / 2 ? 1 : split);
   p.work = (int32_t)(tiles * p.split);
   p.grid = p.work;
-  if (backward && wants_dweight(d, k) && p.grid > kMaxSums) p.grid = kMaxSums;
+}
+// Both parts.  Where the backward call sums for a weight, its workgroups stay for several pieces.
+void cut_both(const twg_norm_rope_t *d, bool backward, PartArgs *p) {
+  for (int k = 0; k < 2; ++k) cut(d, backward, k, p[k]);
+  if (!backward || !wants_dweight(d)) return;
+  const int64_t work = (int64_t)p[0].work + p[1].work, rounds = (work + kMaxSums - 1) / kMaxSums;
+  for (int k = 0; k < 2; ++k)
+    if (p[k].work) p[k].grid = (int32_t)((p[k].work + rounds - 1) / rounds);
 }
 
 template <typename T, typename TW, int V, int C, bool ADJ>
-int launch(const RopeArgs &a, bool backward, hipStream_t s) {
+int launch(const RopeArgs &a, bool backward, bool stream, hipStream_t s) {
   const unsigned grid = (unsigned)(a.part[0].grid + a.part[1].grid);
-  if (backward)
-    rope_backward<T, TW, V, C, ADJ><<<grid, kThreads, 0, s>>>(a);
+  constexpr bool HINT = V * sizeof(T) == 16 && !ADJ;  // (the hint is for pairs in halves only, see run())
+  if (backward && stream && HINT)
+    rope_backward<T, TW, V, C, ADJ, HINT><<<grid, kThreads, 0, s>>>(a);
+  else if (backward)
+    rope_backward<T, TW, V, C, ADJ, false><<<grid, kThreads, 0, s>>>(a);
+  else if (stream && HINT)
+    rope_forward<T, TW, V, C, ADJ, HINT><<<grid, kThreads, 0, s>>>(a);
   else
-    rope_forward<T, TW, V, C, ADJ><<<grid, kThreads, 0, s>>>(a);
+    rope_forward<T, TW, V, C, ADJ, false><<<grid, kThreads, 0, s>>>(a);
   return (int)hipGetLastError();
 }
 
 template <typename T, typename TW>
-int launch_typed(const RopeArgs &a, int v, bool adjacent, bool backward, hipStream_t s) {
+int launch_typed(const RopeArgs &a, int v, bool adjacent, bool backward, bool stream, hipStream_t s) {
 #define TWG_ROPE_V(V, C) \
-  (adjacent ? launch<T, TW, V, C, true>(a, backward, s) : launch<T, TW, V, C, false>(a, backward, s))
+  (adjacent ? launch<T, TW, V, C, true>(a, backward, stream, s) : launch<T, TW, V, C, false>(a, backward, stream, s))
   if constexpr (sizeof(T) == 2)
     if (v == 8) return TWG_ROPE_V(8, 1);
   if (v == 4) return TWG_ROPE_V(4, 1);
@@ -559,16 +591,17 @@ int run(const twg_norm_rope_t *d, bool backward, void *scratch, size_t scratch_b
     a.tokens = (uint32_t)d->tokens;
     a.position_dtype = d->position_dtype;
     a.norm = d->norm != 0;
+    a.n_axes = d->n_axes;
     a.eps = d->eps;
     a.inv_dim = 1.0f / (float)d->head_dim;
     a.positions = d->positions;
     a.inv_freq = d->inv_freq;
     for (int k = 0; k < 3; ++k) a.pos_stride[k] = d->pos_stride[k];
     float *room = static_cast<float *>(scratch);
+    cut_both(d, backward, a.part);
     for (int k = 0; k < 2; ++k) {
       const twg_rope_part_t &p = d->part[k];
       PartArgs &to = a.part[k];
-      cut(d, backward, k, to);
       to.x = p.x;
       to.dy = p.dy;
       to.weight = p.weight;
@@ -587,12 +620,18 @@ int run(const twg_norm_rope_t *d, bool backward, void *scratch, size_t scratch_b
     }
     if ((int64_t)a.part[0].grid + a.part[1].grid > INT32_MAX) return TWG_E_TOO_LARGE;
     for (int i = 0; i < a.rot_pairs; ++i) a.pair_axis[i] = d->pair_axis[i];
+    const double bytes = (double)a.all_tokens * (double)total_heads(d) * d->head_dim * nn_size(d->dtype) * (backward && d->norm ? 3 : 2);
+    // Nontemporal loads and stores where every run of a head is whole 128-byte lines and more is moved
+    // than the last-level cache holds: 32768 tokens x 40 heads of 128, bfloat16, forward 133 -> 121 us,
+    // backward 217 -> 196; with 84 MB 18.0 -> 20.3, with runs of 64 bytes (heads of 64) 67 -> 70.
+    const bool stream = bytes > 256.0 * (1 << 20) && !d->adjacent && d->rot_dim == d->head_dim &&
+                        (d->head_dim / 2 * nn_size(d->dtype)) % 128 == 0;
     rc = nn_dispatch(d->dtype, [&](auto t) {
       using T = decltype(t);
       // weights come in the heads' type or in binary32
       if (d->norm && d->weight_dtype == TWG_DT_F32)
-        return launch_typed<T, float>(a, lanes.v, d->adjacent != 0, backward, s);
-      return launch_typed<T, T>(a, lanes.v, d->adjacent != 0, backward, s);
+        return launch_typed<T, float>(a, lanes.v, d->adjacent != 0, backward, stream, s);
+      return launch_typed<T, T>(a, lanes.v, d->adjacent != 0, backward, stream, s);
     });
     if (rc) return rc;
   }
@@ -619,11 +658,10 @@ int twg_norm_rope_backward(const twg_norm_rope_t *d, void *scratch, size_t scrat
 size_t twg_norm_rope_backward_scratch_bytes(const twg_norm_rope_t *d) {
   if (check(d, true) <= 0 || !wants_dweight(d)) return 0;
   size_t rows = 0;
-  for (int k = 0; k < 2; ++k) {
-    PartArgs p{};
-    cut(d, true, k, p);
-    if (wants_dweight(d, k)) rows += (size_t)p.grid;
-  }
+  PartArgs p[2] = {};
+  cut_both(d, true, p);
+  for (int k = 0; k < 2; ++k)
+    if (wants_dweight(d, k)) rows += (size_t)p[k].grid;
   return rows * (size_t)d->head_dim * sizeof(float);
 }
 

@@ -9,6 +9,7 @@ call fails, an exception is raised.
 import collections
 import ctypes
 import os
+import struct
 
 # torch bundles its own HIP runtime under the same SONAME as /opt/rocm's; it has to
 # be the first one loaded into the process or two runtimes end up side by side.
@@ -164,7 +165,8 @@ def load():
     L.twg_ne_scalar.argtypes = [vp, vp, i32, ctypes.c_double, i64, ip, vp]
     L.twg_and.argtypes = [vp, vp, vp, i32, ip, vp]
     L.twg_abs.argtypes = [vp, vp, i32, ip, vp]
-    rp, lp, u64 = ctypes.POINTER(NormRope), ctypes.POINTER(TokenLogprobsArgs), ctypes.c_uint64
+    # (argument structures: a byref, or the packed bytes that the functions on tensors build)
+    rp, lp, u64 = vp, vp, ctypes.c_uint64
     L.twg_norm_rope.argtypes = [rp, vp]
     L.twg_norm_rope_backward.argtypes = [rp, vp, sz, vp]
     L.twg_norm_rope_backward_scratch_bytes.argtypes = [rp]
@@ -336,69 +338,79 @@ class Event:
 _FLOATS = (torch.float16, torch.bfloat16, torch.float32)
 _POSITIONS = (torch.int32, torch.int64, torch.float32)
 
-
-def _require(ok, message):
-    if not ok:
-        raise ValueError(message)
+# twg_norm_rope_t, twg_rope_part_t and twg_token_logprobs_t, packed in one go: setting the fields of
+# a ctypes structure one by one costs more than the rest of a call
+_ROPE_HEAD = struct.Struct("@8if i 2q P 3q P %ds" % (ROPE_MAX_HEAD_DIM // 2))
+_ROPE_PART = struct.Struct("@q 5P 9q")
+_NO_PART = bytes(_ROPE_PART.size)
+_LOGPROBS = struct.Struct("@2i 3q 2P q f i 9P q")
 
 
 def _stream_for(t):
     """The stream argument for work on t."""
-    if t.device.type == "cuda":
-        _require(t.device.index == 0, "the library is bound to device 0")
-        return torch.cuda.current_stream(t.device).cuda_stream or STREAM_NULL
-    _require(t.device.type == "webgpu", f"expected a tensor in GPU memory, got {t.device}")
+    dev = t.device
+    if dev.type == "cuda":
+        if dev.index != 0:
+            raise ValueError("the library is bound to device 0")
+        return torch._C._cuda_getCurrentRawStream(0) or STREAM_NULL  # torch.cuda.current_stream() takes 2 us
+    if dev.type != "webgpu":
+        raise ValueError(f"expected a tensor in GPU memory, got {dev}")
     return None
 
 
 def _same_device(first, *others):
+    dev = first.device
     for t in others:
-        _require(t is None or t.device == first.device, "all tensors must be on one device")
+        if t is not None and t.device != dev:
+            raise ValueError("all tensors must be on one device")
 
 
 def _ptr(t):
-    return None if t is None else t.data_ptr()
+    return 0 if t is None else t.data_ptr()
 
 
-def _norm_rope_args(q, k, positions, inv_freq, q_weight, k_weight, eps, pair_axis, adjacent):
-    _require(q.dim() == 4 and q.dtype in _FLOATS, "q must be [batch, tokens, heads, head_dim] of float16, bfloat16 or float32")
+def _norm_rope_head(q, k, positions, inv_freq, q_weight, k_weight, eps, pair_axis, adjacent):
+    """The checked arguments that the forward and the backward call share, packed."""
+    dtype = q.dtype
+    if q.dim() != 4 or dtype not in _FLOATS:
+        raise ValueError("q must be [batch, tokens, heads, head_dim] of float16, bfloat16 or float32")
     B, T, _, D = q.shape
-    _require(k is None or (k.dim() == 4 and k.shape[:2] == q.shape[:2] and k.shape[3] == D and k.dtype == q.dtype),
-             "k must have q's dtype and shape up to the number of heads")
-    _require(positions.dim() in (1, 2, 3) and positions.dtype in _POSITIONS,
-             "positions must be [tokens], [batch, tokens] or [axes, batch, tokens] of int32, int64 or float32")
+    if k is not None:
+        ks = k.shape
+        if len(ks) != 4 or ks[0] != B or ks[1] != T or ks[3] != D or k.dtype != dtype:
+            raise ValueError("k must have q's dtype and shape up to the number of heads")
     _same_device(q, k, positions, inv_freq, q_weight, k_weight)
-    _require(inv_freq.dim() == 1 and inv_freq.dtype == torch.float32 and inv_freq.is_contiguous(),
-             "inv_freq must be a contiguous float32 vector, one entry per rotated pair")
-    axes = positions.shape[0] if positions.dim() == 3 else 1
-    _require(tuple(positions.shape) == ((T,), (B, T), (axes, B, T))[positions.dim() - 1], "positions do not fit q")
-    _require(2 * inv_freq.shape[0] <= D <= ROPE_MAX_HEAD_DIM, "more pairs than the head has, or a head beyond 512 elements")
-    _require(1 <= axes <= ROPE_MAX_AXES, "1 to 8 position axes")
-    _require(pair_axis is None or len(pair_axis) == inv_freq.shape[0], "pair_axis must name an axis for each rotated pair")
-    _require(pair_axis is not None or axes == 1, "several position axes need pair_axis")
-    _require(eps is not None or (q_weight is None and k_weight is None), "weights without a norm (eps is None)")
-    d = NormRope()
-    d.dtype = d.weight_dtype = DTYPES[q.dtype]
+    pairs = inv_freq.shape[0] if inv_freq.dim() == 1 else -1
+    if pairs < 0 or inv_freq.dtype != torch.float32 or not inv_freq.is_contiguous():
+        raise ValueError("inv_freq must be a contiguous float32 vector, one entry per rotated pair")
+    if 2 * pairs > D or D > ROPE_MAX_HEAD_DIM:
+        raise ValueError("more pairs than the head has, or a head beyond 512 elements")
+    ps, st, pt = positions.shape, positions.stride(), positions.dtype
+    nd = len(ps)
+    if not 1 <= nd <= 3 or pt not in _POSITIONS or ps[-1] != T or (nd > 1 and ps[-2] != B):
+        raise ValueError("positions must be [tokens], [batch, tokens] or [axes, batch, tokens] of int32, int64 or float32")
+    axes = ps[0] if nd == 3 else 1
+    if not 1 <= axes <= ROPE_MAX_AXES:
+        raise ValueError("1 to 8 position axes")
+    if pair_axis is None:
+        if axes != 1 and pairs:
+            raise ValueError("several position axes need pair_axis")
+    elif len(pair_axis) != pairs:
+        raise ValueError("pair_axis must name an axis for each rotated pair")
+    weight_dtype = dtype
     for w in (q_weight, k_weight):
-        if w is not None:
-            _require(w.shape == (D,) and w.is_contiguous() and w.dtype in (q.dtype, torch.float32),
-                     "a norm weight must be a contiguous vector [head_dim] of q's dtype or float32")
-            d.weight_dtype = DTYPES[w.dtype]
-    _require(q_weight is None or k_weight is None or q_weight.dtype == k_weight.dtype, "norm weights of two dtypes")
-    d.position_dtype = DTYPES[positions.dtype]
-    d.norm, d.eps = (0, 0.0) if eps is None else (1, eps)
-    d.adjacent, d.n_axes, d.head_dim, d.rot_dim = int(adjacent), axes, D, 2 * inv_freq.shape[0]
-    d.batch, d.tokens = B, T
-    d.positions, d.inv_freq = positions.data_ptr(), inv_freq.data_ptr()
-    st = positions.stride()
-    d.pos_stride[:] = ((0, 0) + st, (0,) + st, st)[positions.dim() - 1]
-    if pair_axis is not None:
-        ctypes.memmove(d.pair_axis, bytes(pair_axis), len(pair_axis))
-    for i, (x, w) in enumerate(((q, q_weight), (k, k_weight))):
-        if x is not None:
-            p = d.part[i]
-            p.heads, p.weight = x.shape[2], _ptr(w)
-    return d
+        if w is None:
+            continue
+        if eps is None:
+            raise ValueError("weights without a norm (eps is None)")
+        if w.shape != (D,) or not w.is_contiguous() or (w.dtype != dtype and w.dtype != torch.float32):
+            raise ValueError("a norm weight must be a contiguous vector [head_dim] of q's dtype or float32")
+        weight_dtype = w.dtype
+    if q_weight is not None and k_weight is not None and q_weight.dtype != k_weight.dtype:
+        raise ValueError("norm weights of two dtypes")
+    return _ROPE_HEAD.pack(DTYPES[dtype], DTYPES[weight_dtype], DTYPES[pt], eps is not None, bool(adjacent), axes, D, 2 * pairs,
+                           0.0 if eps is None else eps, 0, B, T, positions.data_ptr(), st[0] if nd == 3 else 0,
+                           st[-2] if nd > 1 else 0, st[-1], inv_freq.data_ptr(), b"" if pair_axis is None else bytes(pair_axis))
 
 
 def _dense_heads(x):
@@ -418,25 +430,27 @@ def norm_rope(q, k, positions, inv_freq, q_weight=None, k_weight=None, eps=1e-6,
     q_out / k_out: where the results go (unit stride along head_dim); q and k themselves for a
     call in place."""
     stream = _stream_for(q)
-    d = _norm_rope_args(q, k, positions, inv_freq, q_weight, k_weight, eps, pair_axis, adjacent)
-    outs = []
-    for i, (x, out) in enumerate(((q, q_out), (k, k_out))):
+    args = _norm_rope_head(q, k, positions, inv_freq, q_weight, k_weight, eps, pair_axis, adjacent)
+    outs, keep = [], []
+    for x, w, out in ((q, q_weight, q_out), (k, k_weight, k_out)):
         if x is None:
-            _require(out is None, "an output without its input")
+            if out is not None:
+                raise ValueError("an output without its input")
+            args += _NO_PART
             outs.append(None)
             continue
+        x = _dense_heads(x)
         if out is None:
             out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
         else:
             _same_device(x, out)
-            _require(out.shape == x.shape and out.dtype == x.dtype and (out.stride(3) == 1 or out.shape[3] == 1),
-                     "an output must have its input's shape and dtype and unit stride along head_dim")
-        x = _dense_heads(x)
-        p = d.part[i]
-        p.x, p.out = x.data_ptr(), out.data_ptr()
-        p.x_stride[:], p.out_stride[:] = x.stride()[:3], out.stride()[:3]
+            if out.shape != x.shape or out.dtype != x.dtype or (out.stride(3) != 1 and out.shape[3] != 1):
+                raise ValueError("an output must have its input's shape and dtype and unit stride along head_dim")
+        args += _ROPE_PART.pack(x.shape[2], x.data_ptr(), 0, out.data_ptr(), _ptr(w), 0, *x.stride()[:3], 0, 0, 0,
+                                *out.stride()[:3])
+        keep.append(x)
         outs.append(out)
-    check(load().twg_norm_rope(ctypes.byref(d), stream))
+    check(load().twg_norm_rope(args, stream))
     return tuple(outs)
 
 
@@ -445,27 +459,30 @@ def norm_rope_backward(dq, dk, q, k, positions, inv_freq, q_weight=None, k_weigh
     """Gradients of norm_rope for the incoming gradients dq and dk of its results:
     (grad q, grad k, grad q_weight, grad k_weight), None for what the call does not have."""
     stream = _stream_for(q)
-    d = _norm_rope_args(q, k, positions, inv_freq, q_weight, k_weight, eps, pair_axis, adjacent)
+    args = _norm_rope_head(q, k, positions, inv_freq, q_weight, k_weight, eps, pair_axis, adjacent)
     grads, keep = [None] * 4, []
     for i, (x, dy, w) in enumerate(((q, dq, q_weight), (k, dk, k_weight))):
         if x is None:
-            _require(dy is None, "a gradient without its input")
+            if dy is not None:
+                raise ValueError("a gradient without its input")
+            args += _NO_PART
             continue
         _same_device(x, dy)
-        _require(dy.shape == x.shape and dy.dtype == x.dtype, "an incoming gradient must have its input's shape and dtype")
+        if dy.shape != x.shape or dy.dtype != x.dtype:
+            raise ValueError("an incoming gradient must have its input's shape and dtype")
         x, dy = _dense_heads(x), _dense_heads(dy)
         keep.append((x, dy))
-        grads[i] = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-        p = d.part[i]
-        p.x, p.dy, p.out = x.data_ptr(), dy.data_ptr(), grads[i].data_ptr()
-        p.x_stride[:], p.dy_stride[:], p.out_stride[:] = x.stride()[:3], dy.stride()[:3], grads[i].stride()[:3]
+        g = grads[i] = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        gw = 0
         if w is not None:
-            grads[2 + i] = torch.empty_like(w)
-            p.dweight = grads[2 + i].data_ptr()
+            grads[2 + i] = torch.empty(w.shape, dtype=w.dtype, device=w.device)
+            gw = grads[2 + i].data_ptr()
+        args += _ROPE_PART.pack(x.shape[2], x.data_ptr(), dy.data_ptr(), g.data_ptr(), _ptr(w), gw, *x.stride()[:3],
+                                *dy.stride()[:3], *g.stride()[:3])
     L = load()
-    need = L.twg_norm_rope_backward_scratch_bytes(ctypes.byref(d))
+    need = L.twg_norm_rope_backward_scratch_bytes(args)
     scratch = torch.empty(need // 4, dtype=torch.float32, device=q.device) if need else None
-    check(L.twg_norm_rope_backward(ctypes.byref(d), _ptr(scratch), need, stream))
+    check(L.twg_norm_rope_backward(args, _ptr(scratch), need, stream))
     return tuple(grads)
 
 
@@ -476,17 +493,12 @@ def _rows(logits):
     return logits if logits.stride(1) == 1 or logits.shape[1] == 1 else logits.contiguous()
 
 
-def _logprob_args(logits, targets, scale, ignore_index):
-    _require(logits.dim() == 2 and logits.dtype in _FLOATS, "logits must be [rows, vocab] of float16, bfloat16 or float32")
-    _require(targets.shape == logits.shape[:1] and targets.dtype in (torch.int32, torch.int64) and targets.is_contiguous(),
-             "targets must be a contiguous int32 or int64 vector, one per row")
+def _check_rows(logits, targets):
+    if logits.dim() != 2 or logits.dtype not in _FLOATS:
+        raise ValueError("logits must be [rows, vocab] of float16, bfloat16 or float32")
+    if targets.shape != logits.shape[:1] or targets.dtype not in (torch.int32, torch.int64) or not targets.is_contiguous():
+        raise ValueError("targets must be a contiguous int32 or int64 vector, one per row")
     _same_device(logits, targets)
-    d = TokenLogprobsArgs()
-    d.dtype, d.target_dtype = DTYPES[logits.dtype], DTYPES[targets.dtype]
-    d.rows, d.vocab = logits.shape
-    d.row_stride, d.logits, d.targets = logits.stride(0), logits.data_ptr(), targets.data_ptr()
-    d.ignore_index, d.scale = ignore_index, scale
-    return d
 
 
 def token_logprobs(logits, targets, top_k=0, scale=1.0, ignore_index=-100):
@@ -495,21 +507,24 @@ def token_logprobs(logits, targets, top_k=0, scale=1.0, ignore_index=-100):
     call takes, and the top_k alternatives (ties: the lowest id first), all float32 but the
     int64 ids.  scale multiplies the logits (one over the temperature); -inf logits are masked."""
     stream = _stream_for(logits)
+    _check_rows(logits, targets)
     logits = _rows(logits)
-    d = _logprob_args(logits, targets, scale, ignore_index)
-    _require(0 <= top_k <= min(LOGPROBS_MAX_TOP_K, d.vocab), "top_k must be in 0..min(64, vocab)")
-    rows, dev = d.rows, logits.device
+    rows, vocab = logits.shape
+    if not 0 <= top_k <= min(LOGPROBS_MAX_TOP_K, vocab):
+        raise ValueError("top_k must be in 0..min(64, vocab)")
+    dev = logits.device
     stats = torch.empty((4, rows), dtype=torch.float32, device=dev)
     top = torch.empty((rows, top_k), dtype=torch.float32, device=dev)
     ids = torch.empty((rows, top_k), dtype=torch.int64, device=dev)
-    base = stats.data_ptr()
-    d.logprob, d.entropy, d.row_max, d.row_sum = (base + 4 * rows * i for i in range(4))
-    d.top_k, d.top_logprobs, d.top_ids = top_k, top.data_ptr(), ids.data_ptr()
+    base, row = stats.data_ptr(), 4 * rows
+    args = _LOGPROBS.pack(DTYPES[logits.dtype], DTYPES[targets.dtype], rows, vocab, logits.stride(0), logits.data_ptr(),
+                          targets.data_ptr(), ignore_index, scale, top_k, base, base + row, base + 2 * row, base + 3 * row,
+                          top.data_ptr(), ids.data_ptr(), 0, 0, 0, 0)
     L = load()
-    need = L.twg_token_logprobs_scratch_bytes(ctypes.byref(d))
+    need = L.twg_token_logprobs_scratch_bytes(args)
     scratch = torch.empty(need // 8, dtype=torch.int64, device=dev) if need else None
-    check(L.twg_token_logprobs(ctypes.byref(d), _ptr(scratch), need, stream))
-    return TokenLogprobs(stats[0], stats[1], stats[2], stats[3], top, ids)
+    check(L.twg_token_logprobs(args, _ptr(scratch), need, stream))
+    return TokenLogprobs(*stats.unbind(), top, ids)
 
 
 def token_logprobs_backward(g_logprob, g_entropy, logits, targets, row_max, row_sum, entropy=None, scale=1.0,
@@ -518,21 +533,20 @@ def token_logprobs_backward(g_logprob, g_entropy, logits, targets, row_max, row_
     None).  row_max, row_sum and entropy come from token_logprobs with the same scale.  out may
     be logits itself."""
     stream = _stream_for(logits)
+    _check_rows(logits, targets)
     src = _rows(logits)
-    d = _logprob_args(src, targets, scale, ignore_index)
     for v in (g_logprob, g_entropy, row_max, row_sum, entropy):
-        _require(v is None or (v.shape == targets.shape and v.dtype == torch.float32 and v.is_contiguous()),
-                 "gradients and statistics must be contiguous float32 vectors, one entry per row")
+        if v is not None and (v.shape != targets.shape or v.dtype != torch.float32 or not v.is_contiguous()):
+            raise ValueError("gradients and statistics must be contiguous float32 vectors, one entry per row")
     _same_device(logits, g_logprob, g_entropy, row_max, row_sum, entropy, out)
     if out is None:
         out = torch.empty(src.shape, dtype=src.dtype, device=src.device)
-    else:
-        _require(out.shape == src.shape and out.dtype == src.dtype and (out.stride(1) == 1 or out.shape[1] == 1),
-                 "out must have the logits' shape and dtype and unit stride along vocab")
-    d.g_logprob, d.g_entropy = _ptr(g_logprob), _ptr(g_entropy)
-    d.row_max, d.row_sum, d.entropy = _ptr(row_max), _ptr(row_sum), _ptr(entropy)
-    d.grad, d.grad_stride = out.data_ptr(), out.stride(0)
-    check(load().twg_token_logprobs_backward(ctypes.byref(d), stream))
+    elif out.shape != src.shape or out.dtype != src.dtype or (out.stride(1) != 1 and out.shape[1] != 1):
+        raise ValueError("out must have the logits' shape and dtype and unit stride along vocab")
+    args = _LOGPROBS.pack(DTYPES[src.dtype], DTYPES[targets.dtype], *src.shape, src.stride(0), src.data_ptr(),
+                          targets.data_ptr(), ignore_index, scale, 0, 0, _ptr(entropy), _ptr(row_max), _ptr(row_sum), 0, 0,
+                          _ptr(g_logprob), _ptr(g_entropy), out.data_ptr(), out.stride(0))
+    check(load().twg_token_logprobs_backward(args, stream))
     return out
 
 
@@ -542,13 +556,16 @@ def dropout(x, p, seed, offset=0, residual=None, out=None, d_offset=None):
     training step takes an offset of its own.  p is rounded to a multiple of 2^-16.  d_offset: an
     int64 tensor of one element, added to offset when the kernel runs (captured graphs)."""
     stream = _stream_for(x)
-    _require(x.dtype in _FLOATS, "x must be float16, bfloat16 or float32")
+    if x.dtype not in _FLOATS:
+        raise ValueError("x must be float16, bfloat16 or float32")
     _same_device(x, residual, out, d_offset)
     if out is None:
         out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
     for t in (residual, out):
-        _require(t is None or (t.shape == x.shape and t.dtype == x.dtype), "x, residual and out must agree in shape and dtype")
-    _require(d_offset is None or (d_offset.dtype == torch.int64 and d_offset.numel() == 1), "d_offset must be one int64")
+        if t is not None and (t.shape != x.shape or t.dtype != x.dtype):
+            raise ValueError("x, residual and out must agree in shape and dtype")
+    if d_offset is not None and (d_offset.dtype != torch.int64 or d_offset.numel() != 1):
+        raise ValueError("d_offset must be one int64")
     if x.is_contiguous() and out.is_contiguous() and (residual is None or residual.is_contiguous()):
         it = dense_iter(x.numel())
     else:
