@@ -423,6 +423,7 @@ int twg_norm_rope_backward(const twg_norm_rope_t *d, void *scratch, size_t scrat
 size_t twg_norm_rope_backward_scratch_bytes(const twg_norm_rope_t *d);
 
 #define TWG_LOGPROBS_MAX_TOP_K 64
+#define TWG_LOGPROBS_MAX_VOCAB (INT64_C(1) << 30)
 
 /* Log probabilities of one given token per row of logits [rows, vocab] (unit stride along
  * vocab, rows row_stride elements apart), with c = scale > 0 (one over the temperature),
@@ -438,7 +439,7 @@ typedef struct twg_token_logprobs {
   int32_t dtype;        /* of logits and grad */
   int32_t target_dtype; /* TWG_DT_I32 or TWG_DT_I64 */
   int64_t rows;
-  int64_t vocab;        /* 1..2^31 - 1 */
+  int64_t vocab;        /* 1..TWG_LOGPROBS_MAX_VOCAB */
   int64_t row_stride;
   const void *logits;
   const void *targets;  /* [rows] */

@@ -123,7 +123,7 @@ def logprobs(**kw):
 
 @pytest.mark.parametrize("change, code", [
     (dict(dtype=7), BAD), (dict(target_dtype=6), BAD), (dict(rows=-1), BAD), (dict(rows=1 << 40), LARGE), (dict(vocab=0), BAD),
-    (dict(vocab=1 << 31), BAD), (dict(scale=0.0), BAD), (dict(scale=-1.0), BAD), (dict(scale=float("nan")), BAD),
+    (dict(vocab=(1 << 30) + 1), BAD), (dict(scale=0.0), BAD), (dict(scale=-1.0), BAD), (dict(scale=float("nan")), BAD),
     (dict(scale=float("inf")), BAD), (dict(logits=None), BAD), (dict(logits=P + 2), BAD), (dict(targets=None), BAD),
     (dict(targets=P + 4), BAD),
 ])

@@ -296,6 +296,71 @@ def test_token_logprobs_targets_out_of_range():
     assert bool((grad[:3] == 0).all())
 
 
+@pytest.mark.parametrize("order", ["rising", "falling", "last lanes", "one wave"])
+@pytest.mark.parametrize("rows, vocab", [(1, 70000), (3, 9000), (300, 9000), (1100, 5000), (2, 1500)])
+def test_token_logprobs_alternatives_in_unkind_orders(rows, vocab, order):
+    """every element a new best, the best at the very end, all of the best in one lane's or one wavefront's elements,
+    and values that tie at the place of the last alternative"""
+    x = torch.linspace(-5, 5, vocab).repeat(rows, 1)
+    if order == "falling":
+        x = x.flip(1).contiguous()
+    elif order == "last lanes":
+        x = torch.zeros(rows, vocab)
+        x[:, 504:512] = torch.arange(8.0) + 1
+        x[:, -12:] = 9.0
+    elif order == "one wave":
+        x = torch.full((rows, vocab), -1.0)
+        x[:, 512:1024] = 2.0
+    t = torch.zeros(rows, dtype=torch.int64)
+    for dtype in (F32, BF16):
+        xd = x.to(dtype)
+        got = capi.token_logprobs(dev(xd), dev(t), top_k=40)
+        assert torch.equal(host(got.top_ids), torch.sort(xd.float(), dim=1, descending=True, stable=True).indices[:, :40])
+
+
+def test_token_logprobs_more_rows_than_one_launch_takes():
+    rows = (1 << 22) + 3
+    x = torch.zeros(rows, 2, dtype=F16)
+    x[:, 1] = (torch.arange(rows) % 7).to(F16)
+    t = (torch.arange(rows) % 2).int()
+    xd, td = dev(x), dev(t)
+    got = capi.token_logprobs(xd, td, top_k=1)
+    lp = torch.log_softmax(x.double(), 1).gather(1, t.long()[:, None])[:, 0]
+    assert float((host(got.logprob).double() - lp).abs().max()) <= 64 * ref.U * 7
+    assert torch.equal(host(got.top_ids)[:, 0], (x[:, 1] > 0).long())
+    grad = host(capi.token_logprobs_backward(dev(torch.ones(rows)), None, xd, td, got.row_max, got.row_sum))
+    p = torch.softmax(x.double(), 1)
+    want = torch.nn.functional.one_hot(t.long(), 2) - p
+    assert float((grad.double() - want).abs().max()) <= 2.0 ** -11 + 2.0 ** -20
+
+
+def test_offsets_beyond_32_bits():
+    """rows and tokens 2^31 and more elements apart"""
+    far = (1 << 31) + 64
+    buf = torch.empty(far + 4096, dtype=F16, device="webgpu")
+    g = torch.Generator().manual_seed(12)
+    x = torch.randn(2, 3000, generator=g).to(F16)
+    rows = buf.as_strided((2, 3000), (far, 1))
+    rows.copy_(dev(x))
+    t = torch.randint(0, 3000, (2,), generator=g)
+    got = capi.token_logprobs(rows, dev(t), top_k=3)
+    want = ref.token_logprobs(x, t, 3)
+    ref.assert_within(host(got.logprob), *want["logprob"])
+    assert torch.equal(host(got.top_ids), want["top_ids"])
+    gl = torch.ones(2)
+    capi.token_logprobs_backward(dev(gl), None, rows, dev(t), got.row_max, got.row_sum, out=rows)
+    ref.assert_within(host(rows.contiguous()), *ref.token_logprobs_backward(gl, None, x, t))
+    q, _, pos, inv_freq, _, wq, _, _, _ = rope_inputs(1, 2, 2, 0, 64, 64, 1, F16, "dense", I64)
+    cache = buf.as_strided((1, 2, 2, 64), (4 * far, far, 128, 1))
+    capi.norm_rope(dev(q), None, dev(pos), dev(inv_freq), dev(wq), q_out=cache)
+    ref.assert_within(host(cache.contiguous()), *ref.norm_rope(q, pos, inv_freq, wq))
+    y = capi.dropout(rows, 0.5, 3, out=rows)
+    keep = ref.keep_mask(6000, 0.5, 3, 0).view(2, 3000)
+    assert bool((host(y.contiguous())[~keep] == 0).all())
+    del buf, rows, cache, y
+    torch.webgpu.empty_cache()
+
+
 def test_token_logprobs_gradient_in_place_and_into_padded_rows():
     g = torch.Generator().manual_seed(4)
     x = torch.randn(5, 1003, generator=g).to(BF16)

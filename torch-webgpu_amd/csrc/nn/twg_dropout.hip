@@ -203,10 +203,9 @@ bool packs_fit(const Geom &g, const void *out, const void *x, const void *res, i
 template <typename T>
 int launch_dropout(T *out, const T *x, const T *res, const Geom &g, const DropArgs &a, hipStream_t s) {
   const int64_t groups = (g.numel + kPer - 1) / kPer, blocks = (groups + kThreads - 1) / kThreads;
-  if (blocks > INT32_MAX) return TWG_E_TOO_LARGE;
+  if (blocks * kThreads > UINT32_MAX) return TWG_E_TOO_LARGE;  // a launch's threads are counted in 32 bits
   if (packs_fit(g, out, x, res, (int)sizeof(T))) {
     const int64_t small = (groups + kDenseThreads - 1) / kDenseThreads;
-    if (small > INT32_MAX) return TWG_E_TOO_LARGE;
     const bool stream = g.numel * (int64_t)sizeof(T) * (res ? 3 : 2) > kStreamBytes, dense = g.ndim <= 1;
     if constexpr (sizeof(T) == 4) {
       if (dense) {

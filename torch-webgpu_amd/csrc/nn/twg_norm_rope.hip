@@ -618,7 +618,8 @@ int run(const twg_norm_rope_t *d, bool backward, void *scratch, size_t scratch_b
         to.os[i] = p.out_stride[i];
       }
     }
-    if ((int64_t)a.part[0].grid + a.part[1].grid > INT32_MAX) return TWG_E_TOO_LARGE;
+    // a launch's threads are counted in 32 bits
+    if (((int64_t)a.part[0].grid + a.part[1].grid) * kThreads > UINT32_MAX) return TWG_E_TOO_LARGE;
     for (int i = 0; i < a.rot_pairs; ++i) a.pair_axis[i] = d->pair_axis[i];
     const double bytes = (double)a.all_tokens * (double)total_heads(d) * d->head_dim * nn_size(d->dtype) * (backward && d->norm ? 3 : 2);
     // Nontemporal loads and stores where every run of a head is whole 128-byte lines and more is moved

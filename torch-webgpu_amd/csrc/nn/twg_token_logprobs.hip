@@ -630,7 +630,7 @@ __global__ void __launch_bounds__(kThreads) logprobs_grad(LogprobArgs a) {
 int check(const twg_token_logprobs_t *d, bool backward) {
   if (!d || !nn_dtype(d->dtype)) return TWG_E_INVALID_ARG;
   if (d->target_dtype != TWG_DT_I32 && d->target_dtype != TWG_DT_I64) return TWG_E_INVALID_ARG;
-  if (d->rows < 0 || d->vocab < 1 || d->vocab > INT32_MAX) return TWG_E_INVALID_ARG;
+  if (d->rows < 0 || d->vocab < 1 || d->vocab > TWG_LOGPROBS_MAX_VOCAB) return TWG_E_INVALID_ARG;
   if (!(d->scale > 0.0f) || std::isinf(d->scale)) return TWG_E_INVALID_ARG;
   if (!backward && (d->top_k < 0 || d->top_k > TWG_LOGPROBS_MAX_TOP_K || d->top_k > d->vocab))
     return TWG_E_INVALID_ARG;
@@ -684,6 +684,33 @@ RowShape shape_of(const twg_token_logprobs_t *d) {
   return RowShape{4, (int)(splits < kMaxSplits ? splits : kMaxSplits)};
 }
 
+// Rows of one launch: its threads, 256 a row at most and more where a row has several workgroups, have
+// to be counted in 32 bits.  More rows go in several launches.
+constexpr int64_t kMaxRows = INT64_C(1) << 22;
+
+template <typename Call>
+int in_slabs(const twg_token_logprobs_t *d, Call call) {
+  const auto past = [](auto *p, int64_t n) { return p ? p + n : p; };
+  for (int64_t r = 0; r < d->rows; r += kMaxRows) {
+    twg_token_logprobs_t part = *d;
+    const int64_t size = nn_size(d->dtype);
+    part.rows = d->rows - r < kMaxRows ? d->rows - r : kMaxRows;
+    part.logits = static_cast<const char *>(d->logits) + r * d->row_stride * size;
+    part.targets = static_cast<const char *>(d->targets) + r * (d->target_dtype == TWG_DT_I64 ? 8 : 4);
+    part.logprob = past(d->logprob, r);
+    part.entropy = past(d->entropy, r);
+    part.row_max = past(d->row_max, r);
+    part.row_sum = past(d->row_sum, r);
+    part.top_logprobs = past(d->top_logprobs, r * d->top_k);
+    part.top_ids = past(d->top_ids, r * d->top_k);
+    part.g_logprob = past(d->g_logprob, r);
+    part.g_entropy = past(d->g_entropy, r);
+    part.grad = past(static_cast<char *>(d->grad), r * d->grad_stride * size);
+    if (const int rc = call(&part)) return rc;
+  }
+  return 0;
+}
+
 size_t scratch_of(const twg_token_logprobs_t *d, int splits) {
   if (splits == 1) return 0;
   const size_t parts = (size_t)d->rows * (size_t)splits;
@@ -698,12 +725,19 @@ using namespace twg;
 extern "C" {
 
 size_t twg_token_logprobs_scratch_bytes(const twg_token_logprobs_t *d) {
-  return check(d, false) <= 0 ? 0 : scratch_of(d, shape_of(d).splits);
+  if (check(d, false) <= 0) return 0;
+  twg_token_logprobs_t last = *d;  // of several launches only the last can have few rows
+  if (d->rows > kMaxRows) last.rows = (d->rows - 1) % kMaxRows + 1;
+  return scratch_of(&last, shape_of(&last).splits);
 }
 
 int twg_token_logprobs(const twg_token_logprobs_t *d, void *scratch, size_t scratch_bytes, twg_stream_t stream) {
   int rc = check(d, false);
   if (rc <= 0) return rc;
+  if (d->rows > kMaxRows) {
+    if (scratch_bytes < twg_token_logprobs_scratch_bytes(d)) return TWG_E_SCRATCH_SMALL;  // before the first launch
+    return in_slabs(d, [&](const twg_token_logprobs_t *part) { return twg_token_logprobs(part, scratch, scratch_bytes, stream); });
+  }
   const RowShape shape = shape_of(d);
   if (shape.splits > 1) {
     if (!scratch || scratch_bytes < scratch_of(d, shape.splits)) return TWG_E_SCRATCH_SMALL;
@@ -741,6 +775,8 @@ int twg_token_logprobs(const twg_token_logprobs_t *d, void *scratch, size_t scra
 int twg_token_logprobs_backward(const twg_token_logprobs_t *d, twg_stream_t stream) {
   int rc = check(d, true);
   if (rc <= 0) return rc;
+  if (d->rows > kMaxRows)
+    return in_slabs(d, [&](const twg_token_logprobs_t *part) { return twg_token_logprobs_backward(part, stream); });
   if ((rc = ensure_init())) return rc;
   LogprobArgs a = args_of(d);
   a.in_max = d->row_max;
@@ -752,7 +788,7 @@ int twg_token_logprobs_backward(const twg_token_logprobs_t *d, twg_stream_t stre
   a.grad_stride = d->grad_stride;
   return nn_dispatch(d->dtype, [&](auto t) {
     using T = decltype(t);
-    const int64_t per = kGradPacks * kThreads * 16 / (int)sizeof(T), most = INT32_MAX / d->rows;
+    const int64_t per = kGradPacks * kThreads * 16 / (int)sizeof(T), most = INT32_MAX / kThreads / d->rows;
     const int64_t chunks = (d->vocab + per - 1) / per;
     a.splits = (int32_t)(chunks < most ? chunks : most);
     const unsigned grid = (unsigned)(d->rows * a.splits);

@@ -287,7 +287,7 @@ Logprobs token_logprobs_run(const at::Tensor &logits, const at::Tensor &targets,
   TORCH_CHECK(logits.dim() >= 1 && logits.sizes().slice(0, logits.dim() - 1) == targets.sizes(),
               "webgpu token_logprobs: targets must be one per row of logits, got ", targets.sizes(), " beside ", logits.sizes());
   const int64_t vocab = logits.size(-1);
-  TORCH_CHECK(vocab >= 1 && vocab <= INT32_MAX, "webgpu token_logprobs: a vocabulary of ", vocab, " entries");
+  TORCH_CHECK(vocab >= 1 && vocab <= TWG_LOGPROBS_MAX_VOCAB, "webgpu token_logprobs: a vocabulary of ", vocab, " entries");
   TORCH_CHECK(top_k >= 0 && top_k <= std::min<int64_t>(vocab, TWG_LOGPROBS_MAX_TOP_K),
               "webgpu token_logprobs: top_k must be in 0..min(", TWG_LOGPROBS_MAX_TOP_K, ", vocab), got ", top_k);
   TORCH_CHECK(scale > 0 && std::isfinite(scale) && (float)scale > 0 && std::isfinite((float)scale),

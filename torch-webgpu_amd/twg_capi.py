@@ -441,7 +441,7 @@ def norm_rope(q, k, positions, inv_freq, q_weight=None, k_weight=None, eps=1e-6,
             continue
         x = _dense_heads(x)
         if out is None:
-            out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+            out = x.new_empty(x.shape)
         else:
             _same_device(x, out)
             if out.shape != x.shape or out.dtype != x.dtype or (out.stride(3) != 1 and out.shape[3] != 1):
@@ -472,10 +472,10 @@ def norm_rope_backward(dq, dk, q, k, positions, inv_freq, q_weight=None, k_weigh
             raise ValueError("an incoming gradient must have its input's shape and dtype")
         x, dy = _dense_heads(x), _dense_heads(dy)
         keep.append((x, dy))
-        g = grads[i] = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        g = grads[i] = x.new_empty(x.shape)
         gw = 0
         if w is not None:
-            grads[2 + i] = torch.empty(w.shape, dtype=w.dtype, device=w.device)
+            grads[2 + i] = w.new_empty(w.shape)
             gw = grads[2 + i].data_ptr()
         args += _ROPE_PART.pack(x.shape[2], x.data_ptr(), dy.data_ptr(), g.data_ptr(), _ptr(w), gw, *x.stride()[:3],
                                 *dy.stride()[:3], *g.stride()[:3])
@@ -540,7 +540,7 @@ def token_logprobs_backward(g_logprob, g_entropy, logits, targets, row_max, row_
             raise ValueError("gradients and statistics must be contiguous float32 vectors, one entry per row")
     _same_device(logits, g_logprob, g_entropy, row_max, row_sum, entropy, out)
     if out is None:
-        out = torch.empty(src.shape, dtype=src.dtype, device=src.device)
+        out = src.new_empty(src.shape)
     elif out.shape != src.shape or out.dtype != src.dtype or (out.stride(1) != 1 and out.shape[1] != 1):
         raise ValueError("out must have the logits' shape and dtype and unit stride along vocab")
     args = _LOGPROBS.pack(DTYPES[src.dtype], DTYPES[targets.dtype], *src.shape, src.stride(0), src.data_ptr(),
@@ -560,7 +560,7 @@ def dropout(x, p, seed, offset=0, residual=None, out=None, d_offset=None):
         raise ValueError("x must be float16, bfloat16 or float32")
     _same_device(x, residual, out, d_offset)
     if out is None:
-        out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        out = x.new_empty(x.shape)
     for t in (residual, out):
         if t is not None and (t.shape != x.shape or t.dtype != x.dtype):
             raise ValueError("x, residual and out must agree in shape and dtype")
