@@ -14,8 +14,8 @@
 // (widen, maximum, multiply-add, exponential, sum, weighted sum), so that 2-byte elements at 6 TB/s keep
 // the vector units busy for three quarters of the time.  4096 x 131072: bfloat16 with 5
 // alternatives 177 us (6.1 TB/s), float32 327 us (6.6 TB/s).  Rows of a few thousand elements are
-// bound by the chain of a row's own steps: first maxima, lists, join.  The backward pass takes 192 us for
-// 2048 x 151643 bfloat16, a quarter of the rows without a gradient (5.7 TB/s).
+// bound by the chain of a row's own steps: first maxima, lists, join.  The backward pass takes 184 us for
+// 2048 x 151643 bfloat16, a quarter of the rows without a gradient (5.9 TB/s).
 #include "twg_nn.h"
 
 namespace twg {
@@ -374,10 +374,11 @@ __global__ void __launch_bounds__(64 * WAVES) logprobs_rows(LogprobArgs a) {
     bar = any ? -INFINITY : value_of_rank(least - (least == 0x80000000u ? 2 : 1));
   };
   // kUnroll packs of this lane, the first one pack `p` + threadIdx.x
-  // A lane looks at few float32 elements per byte, so the next step's are on their way meanwhile
-  // (517 rows of 131072: 67 -> 53 us); with 16-bit elements the registers that
-  // takes cost more (4096 rows of 131072: 188 -> 192 us).
-  constexpr bool AHEAD = sizeof(T) == 4;
+  // The next step's packs are on their way while a lane looks at one step's (517 rows of 131072 float32
+  // with 5 alternatives 67 -> 53 us, 4096 rows of 8192 bfloat16 without 18.6 -> 15.3).  16-bit
+  // elements and alternatives together take too many registers for it (the same with 5 alternatives
+  // 29 -> 33 us).
+  constexpr bool AHEAD = sizeof(T) == 4 || !TOP;
   Pack<T, E> coming[kUnroll];
   auto fetch = [&](int p, auto whole) {
 #pragma unroll
@@ -395,8 +396,7 @@ __global__ void __launch_bounds__(64 * WAVES) logprobs_rows(LogprobArgs a) {
       raw[u] = coming[u];
       in[u] = decltype(whole)::value || p + u * THREADS + (int)threadIdx.x < last;
     }
-    if (AHEAD && decltype(whole)::value && p + kUnroll * THREADS < last)
-      fetch(p + kUnroll * THREADS, std::false_type());
+    if (AHEAD && decltype(whole)::value && p + kUnroll * THREADS < last) fetch(p + kUnroll * THREADS, std::false_type());
     float v[N], most[kUnroll];
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u) {
@@ -596,8 +596,9 @@ __global__ void __launch_bounds__(kThreads) logprobs_grad(LogprobArgs a) {
     const float g = -p * __fmaf_rn(fmaxf(d, -300.0f), h, l);
     return j == t ? g + hit : g;
   };
-  // elements before the gradient's first 16-byte boundary, whole packs, elements behind them
-  const int lead = (int)((-(uintptr_t)grad & 15) / sizeof(T));
+  // elements before the gradient's first line of 128 bytes, whole packs, elements behind them: a line that
+  // two workgroups share, on different XCDs, would be written in two pieces
+  const int lead = (int)((-(uintptr_t)grad & 127) / sizeof(T));
   const int head = lead < a.vocab ? lead : a.vocab;
   const int packs = (a.vocab - head) / E, tail = a.vocab - head - packs * E;
   const bool alike = (((uintptr_t)x ^ (uintptr_t)grad) & 15) == 0;  // the logits' packs are aligned, too
