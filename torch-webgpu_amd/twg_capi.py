@@ -348,17 +348,21 @@ _LOGPROBS = struct.Struct("@2i 3q 2P q f i 9P q")
 
 def _stream_for(t):
     """The stream argument for work on t."""
-    dev = t.device
-    if dev.type == "cuda":
-        if dev.index != 0:
+    if t.is_cuda:
+        if t.get_device() != 0:
             raise ValueError("the library is bound to device 0")
         return torch._C._cuda_getCurrentRawStream(0) or STREAM_NULL  # torch.cuda.current_stream() takes 2 us
-    if dev.type != "webgpu":
-        raise ValueError(f"expected a tensor in GPU memory, got {dev}")
+    if t.device.type != "webgpu":
+        raise ValueError(f"expected a tensor in GPU memory, got {t.device}")
     return None
 
 
 def _same_device(first, *others):
+    if first.is_cuda:  # (cheaper than comparing devices)
+        for t in others:
+            if t is not None and not (t.is_cuda and t.get_device() == 0):
+                raise ValueError("all tensors must be on one device")
+        return
     dev = first.device
     for t in others:
         if t is not None and t.device != dev:
@@ -481,7 +485,7 @@ def norm_rope_backward(dq, dk, q, k, positions, inv_freq, q_weight=None, k_weigh
                                 *dy.stride()[:3], *g.stride()[:3])
     L = load()
     need = L.twg_norm_rope_backward_scratch_bytes(args)
-    scratch = torch.empty(need // 4, dtype=torch.float32, device=q.device) if need else None
+    scratch = q.new_empty(need // 4, dtype=torch.float32) if need else None
     check(L.twg_norm_rope_backward(args, _ptr(scratch), need, stream))
     return tuple(grads)
 
@@ -512,17 +516,16 @@ def token_logprobs(logits, targets, top_k=0, scale=1.0, ignore_index=-100):
     rows, vocab = logits.shape
     if not 0 <= top_k <= min(LOGPROBS_MAX_TOP_K, vocab):
         raise ValueError("top_k must be in 0..min(64, vocab)")
-    dev = logits.device
-    stats = torch.empty((4, rows), dtype=torch.float32, device=dev)
-    top = torch.empty((rows, top_k), dtype=torch.float32, device=dev)
-    ids = torch.empty((rows, top_k), dtype=torch.int64, device=dev)
+    stats = logits.new_empty((4, rows), dtype=torch.float32)
+    top = logits.new_empty((rows, top_k), dtype=torch.float32)
+    ids = logits.new_empty((rows, top_k), dtype=torch.int64)
     base, row = stats.data_ptr(), 4 * rows
     args = _LOGPROBS.pack(DTYPES[logits.dtype], DTYPES[targets.dtype], rows, vocab, logits.stride(0), logits.data_ptr(),
                           targets.data_ptr(), ignore_index, scale, top_k, base, base + row, base + 2 * row, base + 3 * row,
                           top.data_ptr(), ids.data_ptr(), 0, 0, 0, 0)
     L = load()
     need = L.twg_token_logprobs_scratch_bytes(args)
-    scratch = torch.empty(need // 8, dtype=torch.int64, device=dev) if need else None
+    scratch = logits.new_empty(need // 8, dtype=torch.int64) if need else None
     check(L.twg_token_logprobs(args, _ptr(scratch), need, stream))
     return TokenLogprobs(*stats.unbind(), top, ids)
 
