@@ -218,3 +218,12 @@ def test_the_generators_state():
     with pytest.raises(ValueError):
         torch.webgpu.set_rng_state(torch.zeros(3, dtype=torch.uint8))
     torch.webgpu.set_rng_state(before)
+
+
+def test_the_device_context_takes_the_one_device():
+    import torch_webgpu  # noqa: F401
+    for d in (None, 0, "webgpu", "webgpu:0", torch.device("webgpu", 0)):
+        with torch.webgpu.device(d):
+            assert torch.webgpu.current_device() == 0
+    with pytest.raises(ValueError):
+        torch.webgpu.device(1)

@@ -219,6 +219,42 @@ def test_nn_dropout_trains_and_works_in_place():
         F.dropout(xd, 0.4, inplace=True)
 
 
+@pytest.mark.parametrize("reentrant", [False, True])
+def test_a_recomputed_dropout_drops_the_same_elements(reentrant):
+    from torch.utils.checkpoint import checkpoint
+    torch.manual_seed(21)
+    x, dy = torch.randn(500), torch.randn(500)
+    xd = dev(x, True)
+    y = checkpoint(lambda t: F.dropout(t, 0.5), xd, use_reentrant=reentrant)
+    F.dropout(dev(x), 0.5)  # another draw in between
+    y.backward(dev(dy))
+    ref.assert_within(host(y), *ref.dropout(x, 0.5, 21, 0))
+    ref.assert_within(host(xd.grad), *ref.dropout(dy, 0.5, 21, 0))
+
+
+def test_cpu_gradients_in_the_same_process():
+    x = torch.arange(6.0).requires_grad_()
+    (x * x).sum().backward()
+    assert torch.equal(x.grad, 2 * torch.arange(6.0))
+
+
+def test_one_tensor_used_twice_gets_the_sum_of_its_gradients():
+    x = torch.randn(4, 30)
+    t = torch.tensor([1, 2, 3, 4])
+    xd = dev(x, True)
+    h = ops().dropout(xd, 0.25, 1, 1, xd)  # x is the residual, too
+    lp = ops().token_logprobs(h, dev(t))[0]
+    ent = ops().token_logprobs(xd, dev(t))[1]
+    torch.autograd.backward([lp, ent], [dev(torch.ones(4)), dev(torch.ones(4))])
+    x6 = x.double().requires_grad_()
+    keep = ref.keep_mask(120, 0.25, 1, 1).view(4, 30)
+    logp = torch.log_softmax(x6 + keep * x6 / 0.75, -1)
+    plain = torch.log_softmax(x6, -1)
+    (logp.gather(1, t[:, None]).sum() - (plain.exp() * plain).sum()).backward()
+    # three float32 gradients of order 1 added: 100 U each
+    assert float((host(xd.grad).double() - x6.grad).abs().max()) <= 300 * ref.U * 4
+
+
 def test_a_training_step_of_all_of_them_together():
     """q and k heads -> norm and rotation -> residual with dropout -> log probability, entropy -> gradients of the
     inputs and the norm weights; against float64 autograd of the same chain on the CPU."""

@@ -14,8 +14,33 @@ from .. import _C
 __all__ = [
     "is_initialized", "current_device", "device_count", "is_available", "init", "synchronize",
     "empty_cache", "memory_stats", "get_device_name", "get_device_properties", "manual_seed_all",
-    "manual_seed", "initial_seed", "get_rng_state", "set_rng_state",
+    "manual_seed", "initial_seed", "get_rng_state", "set_rng_state", "device", "get_amp_supported_dtype",
 ]
+
+
+# torch.utils.checkpoint saves and restores the generator's state on devices that say this, so that a
+# recomputed dropout drops what the forward pass dropped.
+_initialized = True
+
+
+class device:
+    """`with torch.webgpu.device(0):` there is one device, which is always the current one."""
+
+    def __init__(self, device=None):
+        index = device if isinstance(device, int) or device is None else torch.device(device).index
+        if index not in (None, -1, 0):
+            raise ValueError(f"webgpu has a single device, got index {index}")
+
+    def __enter__(self):
+        return self
+
+    def __exit__(self, *exc):
+        return False
+
+
+def get_amp_supported_dtype():
+    """No op of this backend is autocast; torch asks before it enters a (disabled) autocast region."""
+    return []
 
 
 def init():
