@@ -156,6 +156,41 @@ def test_norm_rope_in_place_and_into_a_wider_buffer():
     assert torch.equal(host(args[0]), host(apart[0])) and torch.equal(host(args[1]), host(apart[1]))
 
 
+def test_norm_rope_weights_off_their_alignment():
+    q, k, pos, inv_freq, _, wq, wk, dq, dk = rope_inputs(2, 6, 4, 2, 64, 64, 1, BF16, "dense", I64)
+    wide = dev(torch.cat((torch.zeros(1, dtype=BF16), wq, wk)))
+    args = [dev(t) for t in (q, k, pos, inv_freq)] + [wide[1:65], wide[65:]]
+    got = capi.norm_rope(*args)
+    ref.assert_within(host(got[0]), *ref.norm_rope(q, pos, inv_freq, wq))
+    grads = capi.norm_rope_backward(dev(dq), dev(dk), *args)
+    for i, (x, w, dy) in enumerate(((q, wq, dq), (k, wk, dk))):
+        dx, dxb, dw, dwb = ref.norm_rope_backward(dy, x, pos, inv_freq, w)
+        ref.assert_within(host(grads[i]), dx, dxb)
+        ref.assert_within(host(grads[2 + i]), dw, dwb)
+
+
+def test_two_streams_at_once():
+    """calls on two of torch's streams share nothing"""
+    g = torch.Generator().manual_seed(31)
+    q, k, pos, inv_freq, _, wq, wk, dq, dk = (t.cuda() if torch.is_tensor(t) else t for t in
+                                              rope_inputs(2, 300, 4, 2, 64, 64, 1, BF16, "packed", I64))
+    x, t = torch.randn(5, 60000, generator=g).cuda(), torch.randint(0, 60000, (5,), generator=g).cuda()
+
+    def work():
+        return [*capi.norm_rope_backward(dq, dk, q, k, pos, inv_freq, wq, wk), *capi.token_logprobs(x, t, top_k=10)]
+
+    alone = work()
+    torch.cuda.synchronize()
+    streams, results = [torch.cuda.Stream() for _ in range(2)], []
+    for _ in range(5):
+        for s in streams:
+            with torch.cuda.stream(s):
+                results.append(work())
+    torch.cuda.synchronize()
+    for r in results:
+        assert all(torch.equal(a, b) for a, b in zip(r, alone))
+
+
 def test_norm_rope_zero_heads_and_special_values():
     q, k, pos, inv_freq, _, wq, wk, dq, dk = rope_inputs(1, 4, 3, 1, 64, 64, 1, F32, "dense", I64)
     q[0, 1, 2] = 0.0         # the norm of nothing: 0 * eps^(-1/2)
@@ -420,6 +455,10 @@ def test_dropout_mask_goes_by_logical_index():
         for out in (None, torch.empty(24, 6, 40).permute(1, 2, 0), torch.empty(6, 40, 26)[..., 1:25]):
             got = capi.dropout(dev(how(x)), 0.3, 11, 2, residual=dev(x), out=dev(out))
             ref.assert_within(host(got), want, bound)
+    flat = dev(torch.cat((torch.zeros(1), x.flatten())))[1:]  # dense, off its alignment
+    want_flat, bound_flat = ref.dropout(x.flatten(), 0.3, 11, 2)
+    ref.assert_within(host(capi.dropout(flat, 0.3, 11, 2)), want_flat, bound_flat)
+    ref.assert_within(host(capi.dropout(flat, 0.3, 11, 2, out=flat)), want_flat, bound_flat)
     wide = dev(torch.full((6, 40, 26), 5.0))
     capi.dropout(dev(x), 0.3, 11, 2, residual=dev(x), out=wide[..., 1:25])
     back = host(wide)

@@ -401,6 +401,8 @@ def _norm_rope_head(q, k, positions, inv_freq, q_weight, k_weight, eps, pair_axi
             raise ValueError("several position axes need pair_axis")
     elif len(pair_axis) != pairs:
         raise ValueError("pair_axis must name an axis for each rotated pair")
+    if eps is not None and not 0.0 <= eps <= 3.4e38:
+        raise ValueError("eps must be finite and not negative")
     weight_dtype = dtype
     for w in (q_weight, k_weight):
         if w is None:
@@ -497,7 +499,9 @@ def _rows(logits):
     return logits if logits.stride(1) == 1 or logits.shape[1] == 1 else logits.contiguous()
 
 
-def _check_rows(logits, targets):
+def _check_rows(logits, targets, scale):
+    if not 0.0 < scale <= 3.4e38:
+        raise ValueError("scale must be positive and finite")
     if logits.dim() != 2 or logits.dtype not in _FLOATS:
         raise ValueError("logits must be [rows, vocab] of float16, bfloat16 or float32")
     if targets.shape != logits.shape[:1] or targets.dtype not in (torch.int32, torch.int64) or not targets.is_contiguous():
@@ -511,7 +515,7 @@ def token_logprobs(logits, targets, top_k=0, scale=1.0, ignore_index=-100):
     call takes, and the top_k alternatives (ties: the lowest id first), all float32 but the
     int64 ids.  scale multiplies the logits (one over the temperature); -inf logits are masked."""
     stream = _stream_for(logits)
-    _check_rows(logits, targets)
+    _check_rows(logits, targets, scale)
     logits = _rows(logits)
     rows, vocab = logits.shape
     if not 0 <= top_k <= min(LOGPROBS_MAX_TOP_K, vocab):
@@ -536,7 +540,7 @@ def token_logprobs_backward(g_logprob, g_entropy, logits, targets, row_max, row_
     None).  row_max, row_sum and entropy come from token_logprobs with the same scale.  out may
     be logits itself."""
     stream = _stream_for(logits)
-    _check_rows(logits, targets)
+    _check_rows(logits, targets, scale)
     src = _rows(logits)
     for v in (g_logprob, g_entropy, row_max, row_sum, entropy):
         if v is not None and (v.shape != targets.shape or v.dtype != torch.float32 or not v.is_contiguous()):
