@@ -377,7 +377,7 @@ int twg_and(void *out, const void *a, const void *b, int32_t elem_size, const tw
  * are.  Inputs may be broadcast (stride 0); outputs must not overlap anything but, in
  * twg_norm_rope, their own input with the same strides (in place). */
 typedef struct twg_rope_part {
-  int64_t heads;        /* 0: this part is absent */
+  int64_t heads;        /* 0: this part is absent; of its pointers only dweight is used */
   const void *x;        /* the heads before norm and rotation */
   const void *dy;       /* backward: gradient of the rotated heads */
   void *out;            /* forward: rotated heads; backward: gradient of x */
@@ -416,7 +416,8 @@ typedef struct twg_norm_rope {
 int twg_norm_rope(const twg_norm_rope_t *d, twg_stream_t stream);
 /* Gradients of the above: dx into part[].out, the weights' into part[].dweight (summed over
  * batch, tokens and heads in a fixed order: equal calls give equal bits).  x are the
- * inputs of the forward call; without the norm x is not read and may be NULL. */
+ * inputs of the forward call; without the norm x is not read and may be NULL.  A dweight that
+ * nothing adds to (no heads, no tokens) becomes zeros. */
 int twg_norm_rope_backward(const twg_norm_rope_t *d, void *scratch, size_t scratch_bytes,
                            twg_stream_t stream);
 /* Bytes of device scratch the backward call needs (0 where no dweight is asked for). */

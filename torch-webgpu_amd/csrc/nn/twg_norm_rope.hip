@@ -438,7 +438,8 @@ __global__ void __launch_bounds__(1024) rope_weight_sum(SumArgs a) {
 
 int64_t total_heads(const twg_norm_rope_t *d) { return d->part[0].heads + d->part[1].heads; }
 
-bool wants_dweight(const twg_norm_rope_t *d, int k) { return d->norm && d->part[k].heads && d->part[k].dweight; }
+// (a part without heads has a weight gradient, too: zeros)
+bool wants_dweight(const twg_norm_rope_t *d, int k) { return d->norm && d->part[k].dweight; }
 bool wants_dweight(const twg_norm_rope_t *d) { return wants_dweight(d, 0) || wants_dweight(d, 1); }
 
 // 0 = nothing to do, 1 = go on, negative = refused
@@ -464,8 +465,9 @@ int check(const twg_norm_rope_t *d, bool backward) {
   const bool none = all == 0 || total_heads(d) == 0;
   const size_t size = (size_t)nn_size(d->dtype), wsize = (size_t)nn_size(d->weight_dtype);
   for (const twg_rope_part_t &p : d->part) {
+    if (d->norm && (p.heads || backward) && !aligned_to(p.dweight, wsize)) return TWG_E_INVALID_ARG;
     if (!p.heads) continue;
-    if (d->norm && (!aligned_to(p.weight, wsize) || !aligned_to(p.dweight, wsize))) return TWG_E_INVALID_ARG;
+    if (d->norm && !aligned_to(p.weight, wsize)) return TWG_E_INVALID_ARG;
     if (all == 0) continue;
     const bool reads_x = !backward || d->norm;
     if (!p.out || (reads_x && !p.x) || (backward && !p.dy)) return TWG_E_INVALID_ARG;
@@ -581,7 +583,7 @@ int run(const twg_norm_rope_t *d, bool backward, void *scratch, size_t scratch_b
   const bool dw = backward && wants_dweight(d);
   if (rc > 0 && dw) {
     const size_t need = twg_norm_rope_backward_scratch_bytes(d);
-    if (!scratch || scratch_bytes < need) return TWG_E_SCRATCH_SMALL;
+    if (need && (!scratch || scratch_bytes < need)) return TWG_E_SCRATCH_SMALL;  // (0: only for a part without heads)
     if (!aligned_to(scratch, 4)) return TWG_E_INVALID_ARG;
   }
   if (rc == 0 && !dw) return 0;
@@ -589,7 +591,7 @@ int run(const twg_norm_rope_t *d, bool backward, void *scratch, size_t scratch_b
   const hipStream_t s = nn_stream(stream);
   SumArgs sums{};
   sums.dim = d->head_dim;
-  for (int k = 0; k < 2; ++k) sums.to[k] = d->part[k].heads ? d->part[k].dweight : nullptr;
+  for (int k = 0; k < 2; ++k) sums.to[k] = d->part[k].dweight;
   if (rc > 0) {
     RopeArgs a{};
     const Lanes lanes = lanes_of(d, backward);
