@@ -458,9 +458,9 @@ at::Tensor aten_dropout_autograd(const at::Tensor &x, double p, bool train) {
 }
 at::Tensor &aten_dropout_(at::Tensor &x, double p, bool train) {
   check_p(p);
+  if (!train || p == 0 || x.numel() == 0) return x;
   TORCH_CHECK(!(x.requires_grad() && at::GradMode::is_enabled()),
               "webgpu dropout_: not in place on a tensor that requires grad; use dropout");
-  if (!train || p == 0 || x.numel() == 0) return x;
   at::assert_no_internal_overlap(x);
   const auto draw = next_draw();
   dropout_into(x, x, at::Tensor(), p, (uint64_t)draw.first, (uint64_t)draw.second);
