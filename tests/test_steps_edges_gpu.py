@@ -4,6 +4,7 @@ import math
 
 import pytest
 import torch
+import torch.nn.functional as F
 
 import steps_ref as ref
 import twg_capi as capi
@@ -64,3 +65,79 @@ def test_a_weight_without_heads_in_a_backward_pass(q_heads, k_heads):
     for heads, w in ((q_heads, wq), (k_heads, wk)):
         grad = host(w.grad)
         assert bool(torch.isfinite(grad).all()) and bool((grad == 0).all()) == (heads == 0)
+
+
+# ------------------------------------------------------------------------- dropout in place
+
+def kept(n, p, seed, offset=0):
+    """what dropout multiplies n elements by"""
+    threshold = math.floor(p * 65536 + 0.5)
+    return ref.keep_mask(n, p, seed, offset).double() * (65536 / (65536 - threshold))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_dropout_in_place_trains(dtype):
+    torch.manual_seed(41)
+    x, dy = torch.randn(30, 21).to(dtype), torch.randn(30, 21).to(dtype)
+    xd = dev(x, True)
+    y = torch.ops.webgpu.dropout(xd, 0.0, 0)  # a tensor with a history
+    version, address = y._version, y.data_ptr()
+    z = torch.nn.Dropout(0.4, inplace=True)(y)
+    assert z is y and y.data_ptr() == address and y._version > version and y.grad_fn is not None
+    ref.assert_within(host(y), *ref.dropout(x, 0.4, 41, 0))
+    y.backward(dev(dy))
+    ref.assert_within(host(xd.grad), *ref.dropout(dy, 0.4, 41, 0))
+
+
+def test_dropout_in_place_on_a_view_of_a_tensor_with_a_history():
+    torch.manual_seed(42)
+    x, dy = torch.randn(6, 10), torch.randn(6, 10)
+    xd = dev(x, True)
+    y = xd * 1.0
+    F.dropout(y[:, 2:7], 0.5, inplace=True)
+    y.backward(dev(dy))
+    times = torch.ones(6, 10, dtype=torch.float64)
+    times[:, 2:7] = kept(30, 0.5, 42).view(6, 5)
+    # products of a float32 with 0, 1 or 2
+    assert torch.equal(host(y).double(), x.double() * times)
+    assert torch.equal(host(xd.grad).double(), dy.double() * times)
+
+
+def test_dropout_in_place_twice_and_second_derivatives():
+    torch.manual_seed(43)
+    x = torch.randn(64)
+    xd = dev(x, True)
+    y = xd * xd
+    F.dropout(F.dropout(y, 0.5, inplace=True), 0.5, inplace=True)
+    times = kept(64, 0.5, 43, 0) * kept(64, 0.5, 43, 1)
+    (g,) = torch.autograd.grad(y, xd, dev(torch.ones(64)), create_graph=True)
+    (gg,) = torch.autograd.grad(g, xd, dev(torch.ones(64)))
+    assert torch.equal(host(g).double(), 2 * x.double() * times)
+    assert torch.equal(host(gg).double(), 2 * times)
+
+
+def test_dropout_in_place_is_seen_by_what_saved_the_tensor():
+    xd = dev(torch.randn(20), True)
+    y = xd * 1.0
+    z = y * y  # saves y
+    F.dropout(y, 0.5, inplace=True)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        z.backward(dev(torch.ones(20)))
+
+
+def test_dropout_in_place_refuses_leaves_before_it_draws():
+    x = torch.randn(4, 6)
+    xd = dev(x, True)
+    state = torch.webgpu.get_rng_state()
+    for leaf in (xd, xd[1:]):
+        with pytest.raises(RuntimeError, match="leaf Variable"):
+            F.dropout(leaf, 0.5, inplace=True)
+    with pytest.raises(RuntimeError):
+        F.dropout(dev(x[:1]).expand(4, 6), 0.5, inplace=True)  # several elements in one place
+    with pytest.raises(RuntimeError):
+        F.dropout(dev(x.double()), 0.5, inplace=True)
+    assert torch.equal(host(xd), x) and torch.equal(torch.webgpu.get_rng_state(), state)
+    torch.manual_seed(44)
+    with torch.no_grad():  # outside of autograd it may
+        F.dropout(xd, 0.5, inplace=True)
+    ref.assert_within(host(xd), *ref.dropout(x, 0.5, 44, 0))

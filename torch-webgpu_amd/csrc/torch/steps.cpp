@@ -5,6 +5,7 @@
 // They have no counterpart in the reference, whose backend registers no autograd formulas
 // (csrc/ops/webgpu_ops.cpp:63-66); these bring their own, at the AutogradPrivateUse1 key.
 #include <ATen/MemoryOverlap.h>
+#include <torch/csrc/autograd/VariableTypeUtils.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/library.h>
 
@@ -456,15 +457,51 @@ at::Tensor aten_dropout_autograd(const at::Tensor &x, double p, bool train) {
   const auto draw = next_draw();
   return Dropout::apply(x, p, draw.first, draw.second, MaybeTensor());
 }
+
+void dropout_in_place(at::Tensor x, double p, std::pair<int64_t, int64_t> draw) {
+  dropout_into(x, x, at::Tensor(), p, (uint64_t)draw.first, (uint64_t)draw.second);
+  x.unsafeGetTensorImpl()->bump_version();
+}
+
+// In place on a tensor with a history, as torch's own in-place operators are: the backward pass needs
+// nothing of x.
+struct DropoutInPlace : torch::autograd::Function<DropoutInPlace> {
+  static at::Tensor forward(AutogradContext *ctx, const at::Tensor &x, double p, int64_t seed, int64_t offset) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    ctx->saved_data["p"] = p;
+    ctx->saved_data["seed"] = seed;
+    ctx->saved_data["offset"] = offset;
+    dropout_in_place(x, p, {seed, offset});
+    ctx->mark_dirty({x});
+    return x;
+  }
+  static variable_list backward(AutogradContext *ctx, variable_list grads) {
+    return {Dropout::apply(grads[0], ctx->saved_data["p"].toDouble(), ctx->saved_data["seed"].toInt(),
+                           ctx->saved_data["offset"].toInt(), MaybeTensor()),
+            Variable(), Variable(), Variable()};
+  }
+};
+
 at::Tensor &aten_dropout_(at::Tensor &x, double p, bool train) {
   check_p(p);
   if (!train || p == 0 || x.numel() == 0) return x;
-  TORCH_CHECK(!(x.requires_grad() && at::GradMode::is_enabled()),
-              "webgpu dropout_: not in place on a tensor that requires grad; use dropout");
   at::assert_no_internal_overlap(x);
-  const auto draw = next_draw();
-  dropout_into(x, x, at::Tensor(), p, (uint64_t)draw.first, (uint64_t)draw.second);
-  x.unsafeGetTensorImpl()->bump_version();
+  dropout_in_place(x, p, next_draw());
+  return x;
+}
+at::Tensor &aten_dropout_autograd_(at::Tensor &x, double p, bool train) {
+  check_p(p);
+  if (!train || p == 0 || x.numel() == 0) return x;
+  at::assert_no_internal_overlap(x);
+  float_dtype(x, "dropout", "x");
+  const bool grad = torch::autograd::compute_requires_grad(x);
+  torch::autograd::check_inplace(x, grad);  // refuses leaves and views of them, before anything is drawn
+  if (grad) {
+    const auto draw = next_draw();
+    DropoutInPlace::apply(x, p, draw.first, draw.second);
+  } else {
+    dropout_in_place(x, p, next_draw());
+  }
   return x;
 }
 
@@ -496,7 +533,7 @@ TORCH_LIBRARY_IMPL(aten, PrivateUse1, m) {
 }
 TORCH_LIBRARY_IMPL(aten, AutogradPrivateUse1, m) {
   m.impl("dropout", TORCH_FN(ops::aten_dropout_autograd));
-  m.impl("dropout_", TORCH_FN(ops::aten_dropout_));
+  m.impl("dropout_", TORCH_FN(ops::aten_dropout_autograd_));
 }
 
 }  // namespace torch_webgpu
