@@ -27,3 +27,96 @@ def test_dropout_that_drops_nothing_returns_its_input(inplace, grad):
                 assert F.dropout(x, 0.0, inplace=inplace) is x
                 assert torch.nn.Dropout(0.5, inplace=inplace).eval()(x) is x
     assert torch.equal(torch.webgpu.get_rng_state(), state)
+
+
+# ------------------------------------------------------------------------- fake tensors, tracing
+
+def fake(*shape, dtype=torch.float32, grad=False):
+    return torch.empty(*shape, dtype=dtype, device="webgpu", requires_grad=grad)
+
+
+@pytest.mark.parametrize("grad", [False, True])
+@pytest.mark.parametrize("inplace", [False, True])
+@pytest.mark.parametrize("mode", [torch.enable_grad, torch.no_grad, torch.inference_mode])
+def test_dropout_of_a_fake_tensor_draws_nothing(inplace, grad, mode):
+    state = torch.webgpu.get_rng_state()
+    with FakeTensorMode(), mode():
+        leaf = fake(3, 4, 8, dtype=torch.bfloat16, grad=grad)
+        x = leaf if inplace and not grad else leaf * 1
+        version = 0 if mode is torch.inference_mode else x._version
+        y = F.dropout(x.transpose(0, 1) if not inplace else x, 0.25, inplace=inplace)
+        assert y.device.type == "webgpu" and y.dtype == torch.bfloat16
+        assert y.shape == ((3, 4, 8) if inplace else (4, 3, 8))
+        if inplace:
+            assert y is x
+            assert mode is torch.inference_mode or x._version > version
+        else:
+            assert y.transpose(0, 1).is_contiguous()
+        assert y.requires_grad == (grad and mode is torch.enable_grad)
+        if y.requires_grad:
+            y.backward(torch.empty_like(y))
+            assert leaf.grad.shape == leaf.shape and leaf.grad.device.type == "webgpu"
+        if inplace and grad and mode is torch.enable_grad:
+            with pytest.raises(RuntimeError, match="leaf Variable"):
+                F.dropout(leaf, 0.25, inplace=True)
+    assert torch.equal(torch.webgpu.get_rng_state(), state)
+
+
+def test_dropout_that_is_refused_draws_nothing():
+    state = torch.webgpu.get_rng_state()
+    x = torch.empty(0, device="webgpu")
+    for p in (-0.1, 1.5, float("nan")):
+        for inplace in (False, True):
+            with pytest.raises((RuntimeError, ValueError)):
+                F.dropout(x, p, inplace=inplace)
+    assert torch.equal(torch.webgpu.get_rng_state(), state)
+
+
+@pytest.mark.parametrize("mode", [torch.enable_grad, torch.inference_mode])
+def test_the_operators_on_fake_tensors(mode):
+    ops = torch.ops.webgpu
+    with FakeTensorMode(), mode():
+        on = mode is torch.enable_grad
+        q = fake(2, 4, 5, 64, dtype=torch.float16, grad=on).transpose(1, 2)  # heads first
+        k = fake(2, 5, 2, 64, dtype=torch.float16, grad=on)
+        w = fake(64, grad=on)
+        pos, inv_freq = torch.arange(5, device="webgpu"), fake(32)
+        yq, yk = ops.norm_rope(q, k, pos, inv_freq, w)
+        assert yq.shape == (2, 5, 4, 64) and yk.shape == (2, 5, 2, 64) and yq.stride() == q.stride()
+        assert yq.dtype == yk.dtype == torch.float16 and yq.device.type == "webgpu"
+        assert ops.norm_rope(q, None, pos, inv_freq)[0].shape == yq.shape
+        odd = fake(1, 3, 2, 64, 2)[..., 0]  # head_dim is not dense: the result's is
+        assert ops.norm_rope(odd, None, pos[:3], inv_freq)[0].stride(3) == 1
+        x = fake(3, 7, 100, dtype=torch.bfloat16, grad=on)
+        t = torch.empty(3, 7, dtype=torch.int64, device="webgpu")
+        lp, h, top, ids = ops.token_logprobs(x, t, top_k=6)
+        assert lp.shape == h.shape == (3, 7) and top.shape == ids.shape == (3, 7, 6)
+        assert lp.dtype == h.dtype == top.dtype == torch.float32 and ids.dtype == torch.int64
+        d = ops.dropout(yk, 0.1, 1, 2, yk)
+        assert d.shape == yk.shape and d.dtype == torch.float16
+        for v in (yq, yk, lp, h, top, ids, d):
+            assert v.device.type == "webgpu"
+            assert v.requires_grad == (on and v is not top and v is not ids)
+        if on:
+            grads = torch.autograd.grad([yq, yk], [q, k, w], [torch.empty_like(yq), torch.empty_like(yk)])
+            assert [g.shape for g in grads] == [q.shape, k.shape, w.shape] and grads[2].dtype == torch.float32
+            assert torch.autograd.grad(lp, x, torch.empty_like(lp), retain_graph=True)[0].shape == x.shape
+            assert torch.autograd.grad(h, x, torch.empty_like(h))[0].dtype == torch.bfloat16
+
+
+def test_a_traced_dropout_is_one_that_draws():
+    """the seed and the offset of the trace are not in the graph: each run of it draws anew"""
+    from torch.fx.experimental.proxy_tensor import make_fx
+    state = torch.webgpu.get_rng_state()
+    with FakeTensorMode():
+        x = fake(8, 8, grad=True)
+
+        def step(x):
+            y = F.dropout(F.dropout(x, 0.5), 0.5)
+            return y, torch.autograd.grad(y, x, torch.ones_like(y))[0]
+
+        graph = make_fx(step)(x)
+        called = [n.target for n in graph.graph.nodes if n.op == "call_function"]
+    ops = torch.ops.webgpu
+    assert called.count(ops._draw_dropout.default) == 2 and called.count(ops._redo_dropout.default) == 2
+    assert torch.equal(torch.webgpu.get_rng_state(), state)

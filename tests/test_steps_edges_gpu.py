@@ -141,3 +141,84 @@ def test_dropout_in_place_refuses_leaves_before_it_draws():
     with torch.no_grad():  # outside of autograd it may
         F.dropout(xd, 0.5, inplace=True)
     ref.assert_within(host(xd), *ref.dropout(x, 0.5, 44, 0))
+
+
+# ------------------------------------------------------------------------------- compiled
+
+def step_inputs():
+    g = torch.Generator().manual_seed(51)
+    q, r = torch.randn(2, 5, 3, 32, generator=g), torch.randn(2, 5, 96, generator=g)
+    t = torch.randint(0, 96, (2, 5), generator=g)
+    return q, r, 1 + 0.3 * torch.randn(32, generator=g), torch.arange(5), torch.rand(16, generator=g), t
+
+
+def step(q, r, w, pos, inv_freq, t):
+    y = torch.ops.webgpu.norm_rope(q, None, pos, inv_freq, w)[0].view(2, 5, 96)
+    h = torch.ops.webgpu.dropout(F.dropout(y, 0.25), 0.5, 9, 1, r)
+    lp, ent, top, ids = torch.ops.webgpu.token_logprobs(h, t, 4)
+    return lp, ent, top, ids, h
+
+
+@pytest.mark.parametrize("backend_name, outputs", [("webgpu_backend", 5), ("aot_eager", 2)])
+def test_a_compiled_step_gives_what_the_eager_one_gives(backend_name, outputs):
+    """(for an output without a gradient the second backend asks for zeros, which the device does not make)"""
+    q, r, w, pos, inv_freq, t = step_inputs()
+
+    def some(*args):
+        return step(*args)[:outputs]
+
+    def run(f, seed):
+        torch.manual_seed(seed)
+        leaves = [dev(q, True), dev(r, True), dev(w, True)]
+        out = f(*leaves, dev(pos), dev(inv_freq), dev(t))
+        grads = torch.autograd.grad(out[:2], leaves, [dev(torch.ones(2, 5))] * 2)
+        return [host(v) for v in (*out, *grads)]
+
+    torch._dynamo.reset()
+    compiled = torch.compile(some, backend=backend_name, fullgraph=True)
+    results = []
+    for seed in (1, 2):  # a compiled graph takes the seed of each run, not of its trace
+        results.append(run(compiled, seed))
+        for a, b in zip(results[-1], run(some, seed)):
+            assert torch.equal(a, b)
+    assert not torch.equal(results[0][0], results[1][0])
+    torch._dynamo.reset()
+
+
+@pytest.mark.parametrize("backend_name", ["webgpu_backend", "aot_eager"])
+def test_a_compiled_dropout_in_place(backend_name):
+    def f(x):
+        y = x * 2.0
+        F.dropout(y, 0.5, inplace=True)
+        return y
+
+    torch._dynamo.reset()
+    compiled = torch.compile(f, backend=backend_name, fullgraph=True)
+    x = torch.randn(64)
+    for seed in (5, 6):
+        torch.manual_seed(seed)
+        xd = dev(x, True)
+        y = compiled(xd)
+        assert torch.equal(host(y).double(), 2 * x.double() * kept(64, 0.5, seed))
+        y.backward(dev(torch.ones(64)))
+        assert torch.equal(host(xd.grad).double(), 2 * kept(64, 0.5, seed))
+    torch._dynamo.reset()
+
+
+def test_a_dispatch_mode_sees_the_operators():
+    from torch.utils._python_dispatch import TorchDispatchMode
+    seen = []
+
+    class Look(TorchDispatchMode):
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            seen.append(func)
+            return func(*args, **(kwargs or {}))
+
+    args = [dev(t, t.is_floating_point()) for t in step_inputs()]
+    with Look():
+        lp = step(*args)[0]
+        lp.backward(dev(torch.ones(2, 5)))
+    ops = torch.ops.webgpu
+    for op in (ops.norm_rope, ops._norm_rope_backward, ops.dropout, ops._draw_dropout, ops._redo_dropout, ops._token_logprobs,
+               ops._token_logprobs_backward):
+        assert op.default in seen, op

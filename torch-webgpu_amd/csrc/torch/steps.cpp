@@ -3,7 +3,11 @@
 // nn.Dropout), which ATen would compose of bernoulli_ and a stored mask.
 //
 // They have no counterpart in the reference, whose backend registers no autograd formulas
-// (csrc/ops/webgpu_ops.cpp:63-66); these bring their own, at the AutogradPrivateUse1 key.
+// (csrc/ops/webgpu_ops.cpp:63-66); these bring their own, at the AutogradPrivateUse1 key.  The
+// formulas reach memory only through the dispatcher (the operators whose names start with an underscore
+// are theirs), so that fake tensors, tracers and dispatch modes see every step; what a step
+// gives for fake tensors is in torch_webgpu/fakes.py.
+#include <ATen/EmptyTensor.h>
 #include <ATen/MemoryOverlap.h>
 #include <torch/csrc/autograd/VariableTypeUtils.h>
 #include <torch/csrc/autograd/custom_function.h>
@@ -62,6 +66,11 @@ void *ptr(const at::Tensor &t) { return t.defined() ? t.data_ptr() : nullptr; }
 
 at::Tensor unit_last(const at::Tensor &t) {
   return t.size(-1) <= 1 || t.stride(-1) == 1 ? t : t.contiguous();
+}
+
+template <typename Fn>
+c10::TypedOperatorHandle<Fn> handle(const char *name) {
+  return c10::Dispatcher::singleton().findSchemaOrThrow(name, "").typed<Fn>();
 }
 
 // A gradient that is itself to be differentiated (create_graph=True) would silently be a constant.
@@ -179,62 +188,86 @@ variable_list norm_rope_run(const RopeInputs &in) {
   return outs;
 }
 
+// Gradients of q, k and their weights; undefined where nothing flows back or nothing is asked for.
+std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> norm_rope_gradients(
+    const MaybeTensor &dq, const MaybeTensor &dk, const at::Tensor &q, const MaybeTensor &k, const at::Tensor &positions,
+    const at::Tensor &inv_freq, const MaybeTensor &q_weight, const MaybeTensor &k_weight, std::optional<double> eps,
+    at::IntArrayRef pair_axis, bool adjacent, bool q_weight_grad, bool k_weight_grad) {
+  const RopeInputs in{q, or_none(k), positions, inv_freq, or_none(q_weight), or_none(k_weight), eps, pair_axis.vec(), adjacent};
+  const at::Tensor *dys[2] = {&or_none(dq), &or_none(dk)}, *xs[2] = {&in.q, &in.k}, *ws[2] = {&in.q_weight, &in.k_weight};
+  const bool weight_grads[2] = {q_weight_grad, k_weight_grad};
+  twg_norm_rope_t d = rope_args(in);
+  at::Tensor out[4];
+  variable_list keep;
+  for (int i = 0; i < 2; ++i) {
+    if (!xs[i]->defined() || !dys[i]->defined()) continue;  // nothing flows back
+    const at::Tensor x = unit_last(*xs[i]), dy = unit_last(*dys[i]);
+    TORCH_CHECK(is_webgpu(dy) && dy.sizes() == x.sizes() && dy.scalar_type() == x.scalar_type(),
+                "webgpu norm_rope: an incoming gradient must have the dtype and shape of its result");
+    at::Tensor dx = heads_like(x);
+    twg_rope_part_t &p = d.part[i];
+    p.heads = x.size(2);
+    p.x = x.data_ptr();
+    p.dy = dy.data_ptr();
+    p.out = dx.data_ptr();
+    p.weight = ptr(*ws[i]);
+    set_strides(p.x_stride, x);
+    set_strides(p.dy_stride, dy);
+    set_strides(p.out_stride, dx);
+    if (weight_grads[i]) {
+      out[2 + i] = at::empty(ws[i]->sizes(), ws[i]->options());
+      p.dweight = out[2 + i].data_ptr();
+    }
+    keep.push_back(x);
+    keep.push_back(dy);
+    out[i] = dx;
+  }
+  const size_t need = twg_norm_rope_backward_scratch_bytes(&d);
+  at::Tensor scratch;
+  if (need) scratch = at::empty({(int64_t)(need / 4)}, in.q.options().dtype(at::kFloat));
+  TWG_CHECK(twg_norm_rope_backward(&d, ptr(scratch), need, nullptr));
+  return {out[0], out[1], out[2], out[3]};
+}
+
+std::vector<at::Tensor> norm_rope(const at::Tensor &q, const MaybeTensor &k, const at::Tensor &positions,
+                                  const at::Tensor &inv_freq, const MaybeTensor &q_weight, const MaybeTensor &k_weight,
+                                  std::optional<double> eps, at::OptionalIntArrayRef pair_axis, bool adjacent);
+
 struct NormRope : torch::autograd::Function<NormRope> {
   static variable_list forward(AutogradContext *ctx, const at::Tensor &q, const MaybeTensor &k, const at::Tensor &positions,
                                const at::Tensor &inv_freq, const MaybeTensor &q_weight, const MaybeTensor &k_weight,
                                std::optional<double> eps, std::vector<int64_t> pair_axis, bool adjacent) {
     at::AutoDispatchBelowADInplaceOrView below;
-    const RopeInputs in{q, or_none(k), positions, inv_freq, or_none(q_weight), or_none(k_weight), eps, pair_axis, adjacent};
-    variable_list outs = norm_rope_run(in);
-    ctx->save_for_backward({in.q, in.k, in.positions, in.inv_freq, in.q_weight, in.k_weight});
+    static const auto op = handle<decltype(norm_rope)>("webgpu::norm_rope");
+    variable_list outs = op.call(q, k, positions, inv_freq, q_weight, k_weight, eps, at::IntArrayRef(pair_axis), adjacent);
+    const at::Tensor &wq = or_none(q_weight), &wk = or_none(k_weight);
+    ctx->save_for_backward({q, or_none(k), positions, inv_freq, wq, wk});
     ctx->saved_data["norm"] = eps.has_value();
     ctx->saved_data["eps"] = eps.value_or(0.0);
     ctx->saved_data["pair_axis"] = pair_axis;
     ctx->saved_data["adjacent"] = adjacent;
     // (needs_input_grad counts the tensors that are there, not the arguments)
-    ctx->saved_data["weight_grads"] = std::vector<int64_t>{in.q_weight.defined() && in.q_weight.requires_grad(),
-                                                           in.k_weight.defined() && in.k_weight.requires_grad()};
+    ctx->saved_data["weight_grads"] =
+        std::vector<int64_t>{wq.defined() && wq.requires_grad(), wk.defined() && wk.requires_grad()};
     ctx->set_materialize_grads(false);
     return outs;
   }
 
   static variable_list backward(AutogradContext *ctx, variable_list grads) {
     once("norm_rope");
+    at::AutoDispatchBelowADInplaceOrView below;
+    static const auto op = handle<decltype(norm_rope_gradients)>("webgpu::_norm_rope_backward");
     const variable_list saved = ctx->get_saved_variables();
-    RopeInputs in{saved[0], saved[1], saved[2], saved[3], saved[4], saved[5], std::nullopt,
-                  ctx->saved_data["pair_axis"].toIntVector(), ctx->saved_data["adjacent"].toBool()};
+    const auto maybe = [](const at::Tensor &t) { return t.defined() ? MaybeTensor(t) : MaybeTensor(); };
+    const std::vector<int64_t> pair_axis = ctx->saved_data["pair_axis"].toIntVector();
     const std::vector<int64_t> weight_grads = ctx->saved_data["weight_grads"].toIntVector();
-    if (ctx->saved_data["norm"].toBool()) in.eps = ctx->saved_data["eps"].toDouble();
-    twg_norm_rope_t d = rope_args(in);
-    variable_list out(9), keep;
-    const at::Tensor *xs[2] = {&in.q, &in.k}, *ws[2] = {&in.q_weight, &in.k_weight};
-    for (int i = 0; i < 2; ++i) {
-      if (!xs[i]->defined() || (int)grads.size() <= i || !grads[i].defined()) continue;  // nothing flows back
-      const at::Tensor x = unit_last(*xs[i]), dy = unit_last(grads[i]);
-      TORCH_CHECK(is_webgpu(dy) && dy.sizes() == x.sizes() && dy.scalar_type() == x.scalar_type(),
-                  "webgpu norm_rope: an incoming gradient must have the dtype and shape of its result");
-      at::Tensor dx = heads_like(x);
-      twg_rope_part_t &p = d.part[i];
-      p.heads = x.size(2);
-      p.x = x.data_ptr();
-      p.dy = dy.data_ptr();
-      p.out = dx.data_ptr();
-      p.weight = ptr(*ws[i]);
-      set_strides(p.x_stride, x);
-      set_strides(p.dy_stride, dy);
-      set_strides(p.out_stride, dx);
-      if (weight_grads[i]) {
-        out[4 + i] = at::empty(ws[i]->sizes(), ws[i]->options());
-        p.dweight = out[4 + i].data_ptr();
-      }
-      keep.push_back(x);
-      keep.push_back(dy);
-      out[i] = dx;
-    }
-    const size_t need = twg_norm_rope_backward_scratch_bytes(&d);
-    at::Tensor scratch;
-    if (need) scratch = at::empty({(int64_t)(need / 4)}, in.q.options().dtype(at::kFloat));
-    TWG_CHECK(twg_norm_rope_backward(&d, ptr(scratch), need, nullptr));
+    std::optional<double> eps;
+    if (ctx->saved_data["norm"].toBool()) eps = ctx->saved_data["eps"].toDouble();
+    const auto g = op.call(maybe(grads[0]), grads.size() > 1 ? maybe(grads[1]) : MaybeTensor(), saved[0], maybe(saved[1]),
+                           saved[2], saved[3], maybe(saved[4]), maybe(saved[5]), eps, pair_axis,
+                           ctx->saved_data["adjacent"].toBool(), weight_grads[0] != 0, weight_grads[1] != 0);
+    variable_list out(9);
+    std::tie(out[0], out[1], out[4], out[5]) = g;
     return out;
   }
 };
@@ -321,39 +354,59 @@ Logprobs token_logprobs_run(const at::Tensor &logits, const at::Tensor &targets,
   return r;
 }
 
+// With the row's maximum and sum, which the gradient takes.
+typedef std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor> SixTensors;
+SixTensors token_logprobs_stats(const at::Tensor &logits, const at::Tensor &targets, int64_t top_k, double scale,
+                                int64_t ignore_index) {
+  const Logprobs r = token_logprobs_run(logits, targets, top_k, scale, ignore_index);
+  return {r.logprob, r.entropy, r.top, r.ids, r.row_max, r.row_sum};
+}
+
+at::Tensor token_logprobs_gradient(const MaybeTensor &g_logprob, const MaybeTensor &g_entropy, const at::Tensor &logits,
+                                   const at::Tensor &targets, const at::Tensor &row_max, const at::Tensor &row_sum,
+                                   const at::Tensor &entropy, double scale, int64_t ignore_index) {
+  const int64_t rows = targets.numel();
+  const at::Tensor x = unit_last(logits.reshape({rows, logits.size(-1)})), t = targets.reshape({rows}).contiguous();
+  const at::Tensor h = entropy.reshape({rows}).contiguous();
+  at::Tensor grad = at::empty(logits.sizes(), logits.options());
+  twg_token_logprobs_t d = logprob_args(x, t, scale, ignore_index);
+  at::Tensor g[2] = {or_none(g_logprob), or_none(g_entropy)};
+  for (at::Tensor &v : g)
+    if (v.defined()) v = v.reshape({rows}).contiguous();
+  d.g_logprob = static_cast<const float *>(ptr(g[0]));
+  d.g_entropy = static_cast<const float *>(ptr(g[1]));
+  d.row_max = static_cast<float *>(row_max.data_ptr());
+  d.row_sum = static_cast<float *>(row_sum.data_ptr());
+  d.entropy = static_cast<float *>(h.data_ptr());
+  d.grad = grad.data_ptr();
+  d.grad_stride = logits.size(-1);
+  TWG_CHECK(twg_token_logprobs_backward(&d, nullptr));
+  return grad;
+}
+
 struct TokenLogprobs : torch::autograd::Function<TokenLogprobs> {
   static variable_list forward(AutogradContext *ctx, const at::Tensor &logits, const at::Tensor &targets, int64_t top_k,
                                double scale, int64_t ignore_index) {
     at::AutoDispatchBelowADInplaceOrView below;
-    const Logprobs r = token_logprobs_run(logits, targets, top_k, scale, ignore_index);
-    ctx->save_for_backward({logits, r.targets, r.row_max, r.row_sum, r.entropy});
+    static const auto op = handle<decltype(token_logprobs_stats)>("webgpu::_token_logprobs");
+    const auto [logprob, entropy, top, ids, row_max, row_sum] = op.call(logits, targets, top_k, scale, ignore_index);
+    ctx->save_for_backward({logits, targets, row_max, row_sum, entropy});
     ctx->saved_data["scale"] = scale;
     ctx->saved_data["ignore_index"] = ignore_index;
     ctx->set_materialize_grads(false);
-    ctx->mark_non_differentiable({r.top, r.ids});
-    return {r.logprob, r.entropy, r.top, r.ids};
+    ctx->mark_non_differentiable({top, ids});
+    return {logprob, entropy, top, ids};
   }
 
   static variable_list backward(AutogradContext *ctx, variable_list grads) {
     once("token_logprobs");
+    at::AutoDispatchBelowADInplaceOrView below;
+    static const auto op = handle<decltype(token_logprobs_gradient)>("webgpu::_token_logprobs_backward");
     const variable_list saved = ctx->get_saved_variables();
-    const at::Tensor &logits = saved[0];
-    const int64_t rows = saved[1].numel();
-    const at::Tensor x = unit_last(logits.reshape({rows, logits.size(-1)}));
-    at::Tensor grad = at::empty(logits.sizes(), logits.options());
-    twg_token_logprobs_t d = logprob_args(x, saved[1], ctx->saved_data["scale"].toDouble(), ctx->saved_data["ignore_index"].toInt());
-    at::Tensor g[2];
-    for (int i = 0; i < 2; ++i)
-      if (grads[i].defined()) g[i] = grads[i].reshape({rows}).contiguous();
-    d.g_logprob = static_cast<const float *>(ptr(g[0]));
-    d.g_entropy = static_cast<const float *>(ptr(g[1]));
-    d.row_max = static_cast<float *>(saved[2].data_ptr());
-    d.row_sum = static_cast<float *>(saved[3].data_ptr());
-    d.entropy = static_cast<float *>(saved[4].data_ptr());
-    d.grad = grad.data_ptr();
-    d.grad_stride = logits.size(-1);
-    TWG_CHECK(twg_token_logprobs_backward(&d, nullptr));
-    return {grad, Variable(), Variable(), Variable(), Variable()};
+    const auto maybe = [](const at::Tensor &t) { return t.defined() ? MaybeTensor(t) : MaybeTensor(); };
+    return {op.call(maybe(grads[0]), maybe(grads[1]), saved[0], saved[1], saved[2], saved[3], saved[4],
+                    ctx->saved_data["scale"].toDouble(), ctx->saved_data["ignore_index"].toInt()),
+            Variable(), Variable(), Variable(), Variable()};
   }
 };
 
@@ -408,15 +461,20 @@ at::Tensor dropout_run(const at::Tensor &x, double p, int64_t seed, int64_t offs
   return out;
 }
 
+at::Tensor dropout(const at::Tensor &x, double p, int64_t seed, int64_t offset, const MaybeTensor &residual) {
+  return dropout_run(x, p, seed, offset, or_none(residual));
+}
+
 struct Dropout : torch::autograd::Function<Dropout> {
   static at::Tensor forward(AutogradContext *ctx, const at::Tensor &x, double p, int64_t seed, int64_t offset,
                             const MaybeTensor &residual) {
     at::AutoDispatchBelowADInplaceOrView below;
+    static const auto op = handle<decltype(dropout)>("webgpu::dropout");
     ctx->saved_data["p"] = p;
     ctx->saved_data["seed"] = seed;
     ctx->saved_data["offset"] = offset;
     ctx->saved_data["residual"] = residual.has_value() && residual->defined();
-    return dropout_run(x, p, seed, offset, or_none(residual));
+    return op.call(x, p, seed, offset, residual);
   }
   static variable_list backward(AutogradContext *ctx, variable_list grads) {
     at::Tensor gx;  // the mask is found again from the seed, the offset and the elements' places
@@ -428,79 +486,134 @@ struct Dropout : torch::autograd::Function<Dropout> {
   }
 };
 
-at::Tensor dropout(const at::Tensor &x, double p, int64_t seed, int64_t offset, const MaybeTensor &residual) {
-  return dropout_run(x, p, seed, offset, or_none(residual));
-}
 at::Tensor dropout_autograd(const at::Tensor &x, double p, int64_t seed, int64_t offset, const MaybeTensor &residual) {
   return Dropout::apply(x, p, seed, offset, residual);
 }
 
-// the seed and offset of the next call that draws from the backend's generator
-std::pair<int64_t, int64_t> next_draw() {
-  std::lock_guard<std::mutex> hold(g_rng_lock);
-  return {(int64_t)g_rng_seed, (int64_t)g_rng_offset++};
-}
+// ---- aten::dropout: the seed and the offset are the backend's generator's.  A call leaves what it drew
+// as a tensor in host memory, {seed, offset}, for its backward pass: a traced graph draws anew in each run.
 
 void check_p(double p) {
   TORCH_CHECK(p >= 0 && p <= 1, "dropout probability has to be between 0 and 1, but got ", p);
 }
 
-at::Tensor aten_dropout(const at::Tensor &x, double p, bool train) {
-  check_p(p);
-  if (!train || p == 0 || x.numel() == 0) return x;
-  const auto draw = next_draw();
-  return dropout_run(x, p, draw.first, draw.second, at::Tensor());
-}
-at::Tensor aten_dropout_autograd(const at::Tensor &x, double p, bool train) {
-  check_p(p);
-  if (!train || p == 0 || x.numel() == 0) return x;
-  const auto draw = next_draw();
-  return Dropout::apply(x, p, draw.first, draw.second, MaybeTensor());
+at::Tensor next_draw() {
+  at::Tensor draw = at::detail::empty_cpu({2}, at::kLong);
+  int64_t *to = draw.mutable_data_ptr<int64_t>();
+  std::lock_guard<std::mutex> hold(g_rng_lock);
+  to[0] = (int64_t)g_rng_seed;
+  to[1] = (int64_t)g_rng_offset++;
+  return draw;
 }
 
-void dropout_in_place(at::Tensor x, double p, std::pair<int64_t, int64_t> draw) {
-  dropout_into(x, x, at::Tensor(), p, (uint64_t)draw.first, (uint64_t)draw.second);
-  x.unsafeGetTensorImpl()->bump_version();
+void dropout_drawn_into(at::Tensor out, const at::Tensor &x, double p, const at::Tensor &draw) {
+  TORCH_CHECK(draw.is_cpu() && draw.scalar_type() == at::kLong && draw.numel() == 2 && draw.is_contiguous(),
+              "webgpu dropout: not what a call drew");
+  const int64_t *from = draw.const_data_ptr<int64_t>();
+  dropout_into(out, x, at::Tensor(), p, (uint64_t)from[0], (uint64_t)from[1]);
 }
+
+std::tuple<at::Tensor, at::Tensor> draw_dropout(const at::Tensor &x, double p) {
+  float_dtype(x, "dropout", "x");  // (refused before anything is drawn)
+  check_p(p);
+  at::Tensor out = at::empty_like(x, x.options(), c10::MemoryFormat::Preserve), draw = next_draw();
+  dropout_drawn_into(out, x, p, draw);
+  return {out, draw};
+}
+at::Tensor draw_dropout_(at::Tensor &x, double p) {
+  float_dtype(x, "dropout", "x");
+  check_p(p);
+  at::assert_no_internal_overlap(x);
+  const at::Tensor draw = next_draw();
+  dropout_drawn_into(x, x, p, draw);
+  return draw;
+}
+at::Tensor redo_dropout(const at::Tensor &x, double p, const at::Tensor &draw) {
+  at::Tensor out = at::empty_like(x, x.options(), c10::MemoryFormat::Preserve);
+  dropout_drawn_into(out, x, p, draw);
+  return out;
+}
+
+variable_list redone(AutogradContext *ctx, const variable_list &grads) {
+  static const auto op = handle<decltype(redo_dropout)>("webgpu::_redo_dropout");
+  return {op.call(grads[0], ctx->saved_data["p"].toDouble(), ctx->get_saved_variables()[0]), Variable(), Variable()};
+}
+
+struct RedoDropout : torch::autograd::Function<RedoDropout> {
+  static at::Tensor forward(AutogradContext *ctx, const at::Tensor &x, double p, const at::Tensor &draw) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    static const auto op = handle<decltype(redo_dropout)>("webgpu::_redo_dropout");
+    ctx->saved_data["p"] = p;
+    ctx->save_for_backward({draw});
+    return op.call(x, p, draw);
+  }
+  static variable_list backward(AutogradContext *ctx, variable_list grads) { return redone(ctx, grads); }
+};
+at::Tensor redo_dropout_autograd(const at::Tensor &x, double p, const at::Tensor &draw) {
+  return RedoDropout::apply(x, p, draw);
+}
+
+struct DrawDropout : torch::autograd::Function<DrawDropout> {
+  static at::Tensor forward(AutogradContext *ctx, const at::Tensor &x, double p) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    static const auto op = handle<decltype(draw_dropout)>("webgpu::_draw_dropout");
+    const auto [out, draw] = op.call(x, p);
+    ctx->saved_data["p"] = p;
+    ctx->save_for_backward({draw});
+    return out;
+  }
+  static variable_list backward(AutogradContext *ctx, variable_list grads) {
+    variable_list g = redone(ctx, grads);
+    return {g[0], Variable()};
+  }
+};
 
 // In place on a tensor with a history, as torch's own in-place operators are: the backward pass needs
 // nothing of x.
-struct DropoutInPlace : torch::autograd::Function<DropoutInPlace> {
-  static at::Tensor forward(AutogradContext *ctx, const at::Tensor &x, double p, int64_t seed, int64_t offset) {
+struct DrawDropoutInPlace : torch::autograd::Function<DrawDropoutInPlace> {
+  static at::Tensor forward(AutogradContext *ctx, at::Tensor x, double p) {
     at::AutoDispatchBelowADInplaceOrView below;
+    static const auto op = handle<decltype(draw_dropout_)>("webgpu::_draw_dropout_");
     ctx->saved_data["p"] = p;
-    ctx->saved_data["seed"] = seed;
-    ctx->saved_data["offset"] = offset;
-    dropout_in_place(x, p, {seed, offset});
+    ctx->save_for_backward({op.call(x, p)});
+    x.unsafeGetTensorImpl()->bump_version();
     ctx->mark_dirty({x});
     return x;
   }
   static variable_list backward(AutogradContext *ctx, variable_list grads) {
-    return {Dropout::apply(grads[0], ctx->saved_data["p"].toDouble(), ctx->saved_data["seed"].toInt(),
-                           ctx->saved_data["offset"].toInt(), MaybeTensor()),
-            Variable(), Variable(), Variable()};
+    variable_list g = redone(ctx, grads);
+    return {g[0], Variable()};
   }
 };
 
+at::Tensor aten_dropout(const at::Tensor &x, double p, bool train) {
+  check_p(p);
+  if (!train || p == 0 || x.numel() == 0) return x;
+  return std::get<0>(draw_dropout(x, p));
+}
+at::Tensor aten_dropout_autograd(const at::Tensor &x, double p, bool train) {
+  check_p(p);
+  if (!train || p == 0 || x.numel() == 0) return x;
+  return DrawDropout::apply(x, p);
+}
 at::Tensor &aten_dropout_(at::Tensor &x, double p, bool train) {
   check_p(p);
   if (!train || p == 0 || x.numel() == 0) return x;
-  at::assert_no_internal_overlap(x);
-  dropout_in_place(x, p, next_draw());
+  draw_dropout_(x, p);
   return x;
 }
 at::Tensor &aten_dropout_autograd_(at::Tensor &x, double p, bool train) {
   check_p(p);
   if (!train || p == 0 || x.numel() == 0) return x;
-  at::assert_no_internal_overlap(x);
-  float_dtype(x, "dropout", "x");
   const bool grad = torch::autograd::compute_requires_grad(x);
   torch::autograd::check_inplace(x, grad);  // refuses leaves and views of them, before anything is drawn
   if (grad) {
-    const auto draw = next_draw();
-    DropoutInPlace::apply(x, p, draw.first, draw.second);
+    DrawDropoutInPlace::apply(x, p);
   } else {
-    dropout_in_place(x, p, next_draw());
+    at::AutoDispatchBelowADInplaceOrView below;
+    static const auto op = handle<decltype(draw_dropout_)>("webgpu::_draw_dropout_");
+    op.call(x, p);
+    x.unsafeGetTensorImpl()->bump_version();
   }
   return x;
 }
@@ -516,16 +629,36 @@ TORCH_LIBRARY_FRAGMENT(webgpu, m) {
       "token_logprobs(Tensor logits, Tensor targets, int top_k=0, float scale=1.0, int ignore_index=-100) -> "
       "(Tensor logprob, Tensor entropy, Tensor top_logprobs, Tensor top_ids)");
   m.def("dropout(Tensor x, float p, int seed, int offset=0, Tensor? residual=None) -> Tensor");
+  m.def(
+      "_norm_rope_backward(Tensor? dq, Tensor? dk, Tensor q, Tensor? k, Tensor positions, Tensor inv_freq, Tensor? q_weight, "
+      "Tensor? k_weight, float? eps, int[] pair_axis, bool adjacent, bool q_weight_grad, bool k_weight_grad) -> "
+      "(Tensor, Tensor, Tensor, Tensor)");
+  m.def(
+      "_token_logprobs(Tensor logits, Tensor targets, int top_k, float scale, int ignore_index) -> "
+      "(Tensor, Tensor, Tensor, Tensor, Tensor, Tensor)");
+  m.def(
+      "_token_logprobs_backward(Tensor? g_logprob, Tensor? g_entropy, Tensor logits, Tensor targets, Tensor row_max, "
+      "Tensor row_sum, Tensor entropy, float scale, int ignore_index) -> Tensor");
+  m.def("_draw_dropout(Tensor x, float p) -> (Tensor, Tensor)", {at::Tag::nondeterministic_seeded});
+  m.def("_draw_dropout_(Tensor(a!) x, float p) -> Tensor", {at::Tag::nondeterministic_seeded});
+  m.def("_redo_dropout(Tensor x, float p, Tensor draw) -> Tensor");
 }
 TORCH_LIBRARY_IMPL(webgpu, PrivateUse1, m) {
   m.impl("norm_rope", TORCH_FN(ops::norm_rope));
   m.impl("token_logprobs", TORCH_FN(ops::token_logprobs));
   m.impl("dropout", TORCH_FN(ops::dropout));
+  m.impl("_norm_rope_backward", TORCH_FN(ops::norm_rope_gradients));
+  m.impl("_token_logprobs", TORCH_FN(ops::token_logprobs_stats));
+  m.impl("_token_logprobs_backward", TORCH_FN(ops::token_logprobs_gradient));
+  m.impl("_draw_dropout", TORCH_FN(ops::draw_dropout));
+  m.impl("_draw_dropout_", TORCH_FN(ops::draw_dropout_));
+  m.impl("_redo_dropout", TORCH_FN(ops::redo_dropout));
 }
 TORCH_LIBRARY_IMPL(webgpu, AutogradPrivateUse1, m) {
   m.impl("norm_rope", TORCH_FN(ops::norm_rope_autograd));
   m.impl("token_logprobs", TORCH_FN(ops::token_logprobs_autograd));
   m.impl("dropout", TORCH_FN(ops::dropout_autograd));
+  m.impl("_redo_dropout", TORCH_FN(ops::redo_dropout_autograd));
 }
 TORCH_LIBRARY_IMPL(aten, PrivateUse1, m) {
   m.impl("dropout", TORCH_FN(ops::aten_dropout));

@@ -55,6 +55,7 @@ def _install_repr():
 
 _install_repr()
 
+from . import fakes  # noqa: E402,F401
 from .compiler.webgpu_compiler import webgpu_backend  # noqa: E402,F401  (python/torch_webgpu/__init__.py:15)
 
 # The reference lists "webgpu_ops" in __all__ (python/torch_webgpu/__init__.py:17) without
