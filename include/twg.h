@@ -364,8 +364,10 @@ int twg_and(void *out, const void *a, const void *b, int32_t elem_size, const tw
  *  - The calls allocate nothing, never wait and keep nothing between calls, so they may be
  *    captured into a graph; where a call needs scratch, the caller brings it, and two calls
  *    that may run at the same time need two.
- *  - TWG_STREAM_NULL names the process's default (null) stream, which an opaque NULL
- *    cannot (NULL is the library's own stream). */
+ *  - TWG_STREAM_NULL names device 0's default (null) stream, which an opaque NULL
+ *    cannot (NULL is the library's own stream).
+ *  - Pointers and streams are device 0's, whatever the calling thread's current device is; it
+ *    is the same after a call as before. */
 #define TWG_STREAM_NULL ((twg_stream_t)1)
 
 #define TWG_ROPE_MAX_HEAD_DIM 512

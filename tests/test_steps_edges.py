@@ -1,5 +1,8 @@
 """norm_rope, token_logprobs and dropout at the edges of what they take, as far as that shows without a GPU:
 calls that do nothing, calls on fake tensors (shapes, types and devices only), refusals."""
+import os
+import subprocess
+
 import pytest
 import torch
 import torch.nn.functional as F
@@ -120,3 +123,18 @@ def test_a_traced_dropout_is_one_that_draws():
     ops = torch.ops.webgpu
     assert called.count(ops._draw_dropout.default) == 2 and called.count(ops._redo_dropout.default) == 2
     assert torch.equal(torch.webgpu.get_rng_state(), state)
+
+
+# ------------------------------------------------------------------------- the current device
+
+def test_launches_go_to_the_bound_device(tmp_path):
+    """tests/native/current_device_check.cpp: entry points called while another device is current"""
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    rocm = os.environ.get("ROCM_PATH", "/opt/rocm")
+    libs = os.path.join(root, "torch-webgpu_amd", "torch_webgpu")
+    exe = tmp_path / "check"
+    subprocess.run(["g++", "-std=c++17", "-D__HIP_PLATFORM_AMD__", "-I", os.path.join(root, "include"), "-I", os.path.join(rocm, "include"),
+                    os.path.join(root, "tests", "native", "current_device_check.cpp"), "-o", str(exe), "-L", libs, "-ltwg_hip",
+                    "-Wl,-rpath," + libs, "-Wl,-rpath-link," + os.path.join(rocm, "lib")], check=True)
+    done = subprocess.run([str(exe)], stdout=subprocess.PIPE, text=True, timeout=120)
+    assert done.returncode == 0 and "every launch on device 0" in done.stdout, done.stdout

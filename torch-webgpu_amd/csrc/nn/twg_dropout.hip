@@ -264,7 +264,8 @@ extern "C" int twg_dropout(void *out, const void *x, const void *residual, int32
     return TWG_E_INVALID_ARG;
   for (int d = 0; d < g.ndim; ++d)  // several elements in one place: no order among their stores
     if (g.stride[TWG_OUT][d] == 0) return TWG_E_INVALID_ARG;
-  if ((rc = ensure_init())) return rc;
+  const OnBoundDevice device;
+  if ((rc = device.status())) return rc;
   DropArgs a;
   a.seed = seed;
   a.offset = offset;

@@ -587,7 +587,8 @@ int run(const twg_norm_rope_t *d, bool backward, void *scratch, size_t scratch_b
     if (!aligned_to(scratch, 4)) return TWG_E_INVALID_ARG;
   }
   if (rc == 0 && !dw) return 0;
-  if (int e = ensure_init()) return e;
+  const OnBoundDevice device;
+  if (int e = device.status()) return e;
   const hipStream_t s = nn_stream(stream);
   SumArgs sums{};
   sums.dim = d->head_dim;

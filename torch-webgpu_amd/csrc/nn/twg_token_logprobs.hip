@@ -751,7 +751,8 @@ int twg_token_logprobs(const twg_token_logprobs_t *d, void *scratch, size_t scra
     if (!scratch || scratch_bytes < scratch_of(d, shape.splits)) return TWG_E_SCRATCH_SMALL;
     if (!aligned_to(scratch, 8)) return TWG_E_INVALID_ARG;
   }
-  if ((rc = ensure_init())) return rc;
+  const OnBoundDevice device;
+  if ((rc = device.status())) return rc;
   LogprobArgs a = args_of(d);
   a.splits = shape.splits;
   a.scratch = static_cast<uint64_t *>(scratch);
@@ -785,7 +786,8 @@ int twg_token_logprobs_backward(const twg_token_logprobs_t *d, twg_stream_t stre
   if (rc <= 0) return rc;
   if (d->rows > kMaxRows)
     return in_slabs(d, [&](const twg_token_logprobs_t *part) { return twg_token_logprobs_backward(part, stream); });
-  if ((rc = ensure_init())) return rc;
+  const OnBoundDevice device;
+  if ((rc = device.status())) return rc;
   LogprobArgs a = args_of(d);
   a.in_max = d->row_max;
   a.in_sum = d->row_sum;
