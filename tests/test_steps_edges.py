@@ -138,3 +138,26 @@ def test_launches_go_to_the_bound_device(tmp_path):
                     "-Wl,-rpath," + libs, "-Wl,-rpath-link," + os.path.join(rocm, "lib")], check=True)
     done = subprocess.run([str(exe)], stdout=subprocess.PIPE, text=True, timeout=120)
     assert done.returncode == 0 and "every launch on device 0" in done.stdout, done.stdout
+
+
+# -------------------------------------------------------------- the functions on tensors and autograd
+
+def test_the_functions_on_tensors_refuse_what_they_would_not_differentiate():
+    import twg_capi as capi
+    with FakeTensorMode():
+        q, k, w, f = fake(1, 2, 3, 8), fake(1, 2, 1, 8), fake(8), fake(4)
+        pos, x, t, g = torch.arange(2, device="webgpu"), fake(2, 5), torch.zeros(2, dtype=torch.int64, device="webgpu"), fake(2)
+
+        def on(t):
+            return t.clone().requires_grad_()
+
+        calls = [lambda: capi.norm_rope(on(q), k, pos, f, w, w), lambda: capi.norm_rope(q, on(k), pos, f, w, w),
+                 lambda: capi.norm_rope(q, k, pos, f, on(w), w), lambda: capi.norm_rope(q, k, pos, f, w, on(w)),
+                 lambda: capi.norm_rope(q, k, pos, on(f)), lambda: capi.norm_rope(q, k, pos, f, q_out=on(q)),
+                 lambda: capi.norm_rope_backward(on(q), k, q, k, pos, f), lambda: capi.token_logprobs(on(x), t),
+                 lambda: capi.token_logprobs_backward(on(g), None, x, t, g, g),
+                 lambda: capi.token_logprobs_backward(g, None, x, t, g, g, out=on(x)), lambda: capi.dropout(on(x), 0.5, 1),
+                 lambda: capi.dropout(x, 0.5, 1, residual=on(x)), lambda: capi.dropout(x, 0.5, 1, out=on(x))]
+        for call in calls:
+            with pytest.raises(ValueError, match="no gradient is recorded"):
+                call()

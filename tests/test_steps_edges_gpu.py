@@ -222,3 +222,48 @@ def test_a_dispatch_mode_sees_the_operators():
     for op in (ops.norm_rope, ops._norm_rope_backward, ops.dropout, ops._draw_dropout, ops._redo_dropout, ops._token_logprobs,
                ops._token_logprobs_backward):
         assert op.default in seen, op
+
+
+# -------------------------------------------------------------- the functions on tensors and autograd
+
+@pytest.mark.parametrize("device", ["webgpu", "cuda"])
+def test_the_functions_on_tensors_count_what_they_write(device):
+    """with inputs that require grad, where gradients are not recorded"""
+    g = torch.Generator().manual_seed(61)
+    q = torch.randn(1, 4, 2, 32, generator=g).to(device).requires_grad_()
+    w = torch.ones(32).to(device).requires_grad_()
+    x = torch.randn(3, 40, generator=g).to(device).requires_grad_()
+    t, gl = torch.arange(3).to(device), torch.ones(3).to(device)
+    pos, f = torch.arange(4).to(device), torch.rand(16, generator=g).to(device)
+    with torch.no_grad():
+        apart = capi.norm_rope(q, None, pos, f, w)[0]
+        versions = [v._version for v in (q, w, x, apart)]
+        capi.norm_rope(q, None, pos, f, w, q_out=q)
+        assert torch.equal(host(q), host(apart))
+        got = capi.token_logprobs(x, t)
+        assert [v._version for v in (q, w, x, apart)] == [versions[0] + 1, *versions[1:]]
+        capi.dropout(x, 0.5, 1, out=x)
+        capi.token_logprobs_backward(gl, None, x, t, got.row_max, got.row_sum, out=x)
+        assert x._version == versions[2] + 2
+    with torch.inference_mode():
+        y = x * 1.0
+        capi.dropout(y, 0.5, 1, out=y)  # (a tensor without a version)
+
+
+class _Dropout(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x):
+        return capi.dropout(x, 0.5, 7)
+
+    @staticmethod
+    def backward(ctx, g):
+        return capi.dropout(g, 0.5, 7)
+
+
+def test_the_functions_on_tensors_in_an_autograd_function():
+    x = torch.randn(5, 8)
+    xd = dev(x, True)
+    y = _Dropout.apply(xd)
+    y.backward(dev(torch.ones(5, 8)))
+    times = kept(40, 0.5, 7).view(5, 8)
+    assert torch.equal(host(y).double(), x.double() * times) and torch.equal(host(xd.grad).double(), times)

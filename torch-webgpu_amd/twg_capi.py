@@ -13,7 +13,8 @@ import struct
 
 # torch bundles its own HIP runtime under the same SONAME as /opt/rocm's; it has to
 # be the first one loaded into the process or two runtimes end up side by side.
-import torch  # noqa: F401
+import torch
+from torch.autograd.graph import increment_version
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "torch_webgpu", "libtwg_hip.so")
@@ -333,7 +334,10 @@ class Event:
 # "webgpu" device (the work goes to the library's stream) or of PyTorch-ROCm's device 0 (it goes
 # to torch's current stream, so it is ordered with torch's own products there and can be
 # captured with them).  Results and scratch are allocated with torch on the same device.
-# Arguments are checked here; what the library refuses raises TwgError.
+# Arguments are checked here; what the library refuses raises TwgError.  Nothing is recorded for autograd:
+# an input that requires grad is refused while gradients are recorded, so that none is lost in silence
+# (call under torch.no_grad(), or in a torch.autograd.Function whose backward calls the _backward form);
+# a tensor that is written to has its version counted, as after torch's own in-place operators.
 
 _FLOATS = (torch.float16, torch.bfloat16, torch.float32)
 _POSITIONS = (torch.int32, torch.int64, torch.float32)
@@ -367,6 +371,16 @@ def _same_device(first, *others):
     for t in others:
         if t is not None and t.device != dev:
             raise ValueError("all tensors must be on one device")
+
+
+def _refuse_unrecorded():
+    raise ValueError("no gradient is recorded here for a tensor that requires grad: call under torch.no_grad(), "
+                     "or in a torch.autograd.Function with the _backward form")
+
+
+def _written(t):
+    if t is not None and not t.is_inference():
+        increment_version(t)
 
 
 def _ptr(t):
@@ -436,6 +450,11 @@ def norm_rope(q, k, positions, inv_freq, q_weight=None, k_weight=None, eps=1e-6,
     q_out / k_out: where the results go (unit stride along head_dim); q and k themselves for a
     call in place."""
     stream = _stream_for(q)
+    if torch.is_grad_enabled() and (  # (written out: a loop over the tensors takes longer)
+            q.requires_grad or inv_freq.requires_grad or positions.requires_grad or (k is not None and k.requires_grad)
+            or (q_weight is not None and q_weight.requires_grad) or (k_weight is not None and k_weight.requires_grad)
+            or (q_out is not None and q_out.requires_grad) or (k_out is not None and k_out.requires_grad)):
+        _refuse_unrecorded()
     args = _norm_rope_head(q, k, positions, inv_freq, q_weight, k_weight, eps, pair_axis, adjacent)
     outs, keep = [], []
     for x, w, out in ((q, q_weight, q_out), (k, k_weight, k_out)):
@@ -445,18 +464,25 @@ def norm_rope(q, k, positions, inv_freq, q_weight=None, k_weight=None, eps=1e-6,
             args += _NO_PART
             outs.append(None)
             continue
-        x = _dense_heads(x)
+        shape, strides = x.shape, x.stride()
+        H, D = shape[2:]
+        if strides[3] != 1 and D != 1:
+            x = x.contiguous()
+            strides = x.stride()
         if out is None:
-            out = x.new_empty(x.shape)
+            out = x.new_empty(shape)
+            to = (shape[1] * H * D, H * D, D)
         else:
             _same_device(x, out)
-            if out.shape != x.shape or out.dtype != x.dtype or (out.stride(3) != 1 and out.shape[3] != 1):
+            to = out.stride()
+            if out.shape != shape or out.dtype != x.dtype or (to[3] != 1 and D != 1):
                 raise ValueError("an output must have its input's shape and dtype and unit stride along head_dim")
-        args += _ROPE_PART.pack(x.shape[2], x.data_ptr(), 0, out.data_ptr(), _ptr(w), 0, *x.stride()[:3], 0, 0, 0,
-                                *out.stride()[:3])
+        args += _ROPE_PART.pack(H, x.data_ptr(), 0, out.data_ptr(), _ptr(w), 0, *strides[:3], 0, 0, 0, *to[:3])
         keep.append(x)
         outs.append(out)
     check(load().twg_norm_rope(args, stream))
+    _written(q_out)
+    _written(k_out)
     return tuple(outs)
 
 
@@ -465,6 +491,8 @@ def norm_rope_backward(dq, dk, q, k, positions, inv_freq, q_weight=None, k_weigh
     """Gradients of norm_rope for the incoming gradients dq and dk of its results:
     (grad q, grad k, grad q_weight, grad k_weight), None for what the call does not have."""
     stream = _stream_for(q)
+    if torch.is_grad_enabled() and ((dq is not None and dq.requires_grad) or (dk is not None and dk.requires_grad)):
+        _refuse_unrecorded()
     args = _norm_rope_head(q, k, positions, inv_freq, q_weight, k_weight, eps, pair_axis, adjacent)
     grads, keep = [None] * 4, []
     for i, (x, dy, w) in enumerate(((q, dq, q_weight), (k, dk, k_weight))):
@@ -515,6 +543,8 @@ def token_logprobs(logits, targets, top_k=0, scale=1.0, ignore_index=-100):
     call takes, and the top_k alternatives (ties: the lowest id first), all float32 but the
     int64 ids.  scale multiplies the logits (one over the temperature); -inf logits are masked."""
     stream = _stream_for(logits)
+    if logits.requires_grad and torch.is_grad_enabled():
+        _refuse_unrecorded()
     _check_rows(logits, targets, scale)
     logits = _rows(logits)
     rows, vocab = logits.shape
@@ -540,8 +570,11 @@ def token_logprobs_backward(g_logprob, g_entropy, logits, targets, row_max, row_
     None).  row_max, row_sum and entropy come from token_logprobs with the same scale.  out may
     be logits itself."""
     stream = _stream_for(logits)
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (g_logprob, g_entropy, out)):
+        _refuse_unrecorded()
     _check_rows(logits, targets, scale)
     src = _rows(logits)
+    given = out
     for v in (g_logprob, g_entropy, row_max, row_sum, entropy):
         if v is not None and (v.shape != targets.shape or v.dtype != torch.float32 or not v.is_contiguous()):
             raise ValueError("gradients and statistics must be contiguous float32 vectors, one entry per row")
@@ -554,6 +587,7 @@ def token_logprobs_backward(g_logprob, g_entropy, logits, targets, row_max, row_
                           targets.data_ptr(), ignore_index, scale, 0, 0, _ptr(entropy), _ptr(row_max), _ptr(row_sum), 0, 0,
                           _ptr(g_logprob), _ptr(g_entropy), out.data_ptr(), out.stride(0))
     check(load().twg_token_logprobs_backward(args, stream))
+    _written(given)
     return out
 
 
@@ -565,7 +599,11 @@ def dropout(x, p, seed, offset=0, residual=None, out=None, d_offset=None):
     stream = _stream_for(x)
     if x.dtype not in _FLOATS:
         raise ValueError("x must be float16, bfloat16 or float32")
+    if torch.is_grad_enabled() and (x.requires_grad or (residual is not None and residual.requires_grad)
+                                    or (out is not None and out.requires_grad)):
+        _refuse_unrecorded()
     _same_device(x, residual, out, d_offset)
+    given = out
     if out is None:
         out = x.new_empty(x.shape)
     for t in (residual, out):
@@ -579,4 +617,5 @@ def dropout(x, p, seed, offset=0, residual=None, out=None, d_offset=None):
         it = make_iter(x.shape, out.stride(), x.stride(), None if residual is None else residual.stride())
     check(load().twg_dropout(out.data_ptr(), x.data_ptr(), _ptr(residual), DTYPES[x.dtype], p, seed & (2 ** 64 - 1),
                              offset & (2 ** 64 - 1), _ptr(d_offset), ctypes.byref(it), stream))
+    _written(given)
     return out
