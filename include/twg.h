@@ -437,7 +437,8 @@ size_t twg_norm_rope_backward_scratch_bytes(const twg_norm_rope_t *d);
  *   top_logprobs / top_ids [rows, top_k]: the largest entries in descending order, the lowest
  *             id first among equals (NaN ranks above everything)
  * -inf entries are masked: p = 0, no contribution.  A row with nothing else (s = 0) has
- * logprob and top_logprobs -inf and entropy 0.  +inf or NaN in a row makes its results NaN. */
+ * logprob and top_logprobs -inf and entropy 0.  +inf or NaN in a row makes its results NaN but for
+ * m, which is NaN where the row holds one and +inf otherwise, and the ids. */
 typedef struct twg_token_logprobs {
   int32_t dtype;        /* of logits and grad */
   int32_t target_dtype; /* TWG_DT_I32 or TWG_DT_I64 */

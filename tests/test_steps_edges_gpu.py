@@ -267,3 +267,28 @@ def test_the_functions_on_tensors_in_an_autograd_function():
     y.backward(dev(torch.ones(5, 8)))
     times = kept(40, 0.5, 7).view(5, 8)
     assert torch.equal(host(y).double(), x.double() * times) and torch.equal(host(xd.grad).double(), times)
+
+
+# ---------------------------------------------------------------------- rows that are not finite
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("rows, vocab", [(4, 40000), (5, 500), (600, 9000)])
+def test_the_maximum_of_a_row_that_is_not_finite(rows, vocab, dtype):
+    """NaN where the row holds one, wherever it stands, +inf in a row of others; gradients by the formula"""
+    g = torch.Generator().manual_seed(vocab)
+    x = (torch.randn(rows, vocab, generator=g) * 2).to(dtype)
+    x[0, vocab - 1] = math.nan
+    x[1] = -math.inf
+    x[1, 3] = math.nan
+    x[2, 5], x[2, 77] = math.inf, math.nan
+    x[3, vocab // 2] = math.inf
+    t = torch.arange(rows)
+    xd, td = dev(x), dev(t)
+    got = capi.token_logprobs(xd, td, top_k=3)
+    m = host(got.row_max)
+    assert bool(torch.isnan(m[:3]).all()) and float(m[3]) == math.inf
+    assert torch.equal(m[4:], x[4:].float().amax(1))
+    for v in (got.logprob, got.entropy, got.row_sum, got.top_logprobs):
+        assert bool(torch.isnan(host(v)[:4]).all()) and not bool(torch.isnan(host(v)[4:]).any())
+    grad = host(capi.token_logprobs_backward(dev(torch.ones(rows)), None, xd, td, got.row_max, got.row_sum))
+    assert bool(torch.isnan(grad[:4]).all()) and not bool(torch.isnan(grad[4:]).any())

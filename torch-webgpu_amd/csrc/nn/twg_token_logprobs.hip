@@ -152,6 +152,9 @@ __device__ __forceinline__ void put_top(const LogprobArgs &a, int64_t row, int k
   if (a.top_logprobs) a.top_logprobs[row * a.top_k + k] = log_prob(value_of(key), r, a.scale);
 }
 
+// (fmaxf would leave NaN out)
+__device__ __forceinline__ float max_or_nan(float a, float b) { return a != a || a > b ? a : b; }
+
 // Any row, by its definition: one pass for the maximum, one for the sums, one for each alternative.
 // For rows that the single pass cannot do: nothing but entries near the type's limits,
 // infinities, NaN.  `room`: LDS for one value per wavefront, two of them.
@@ -161,12 +164,12 @@ __device__ void slow_row(const LogprobArgs &a, int64_t row, uint64_t (*room)[WAV
   const int wave = threadIdx.x >> 6;
   float *f0 = (float *)room[0], *f1 = (float *)room[1];
   float m = -INFINITY;
-  for (int i = threadIdx.x; i < a.vocab; i += 64 * WAVES) m = fmaxf(m, (float)x[i]);
-  for (int i = 1; i < 64; i <<= 1) m = fmaxf(m, __shfl_xor(m, i));
+  for (int i = threadIdx.x; i < a.vocab; i += 64 * WAVES) m = max_or_nan(m, (float)x[i]);
+  for (int i = 1; i < 64; i <<= 1) m = max_or_nan(m, __shfl_xor(m, i));
   __syncthreads();
   if ((threadIdx.x & 63) == 0) f0[wave] = m;
   __syncthreads();
-  for (int i = 0; i < WAVES; ++i) m = fmaxf(m, f0[i]);
+  for (int i = 0; i < WAVES; ++i) m = max_or_nan(m, f0[i]);
   float s = 0.0f, t = 0.0f;
   for (int i = threadIdx.x; i < a.vocab; i += 64 * WAVES) {
     const float v = (float)x[i];
