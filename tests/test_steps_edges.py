@@ -161,3 +161,38 @@ def test_the_functions_on_tensors_refuse_what_they_would_not_differentiate():
         for call in calls:
             with pytest.raises(ValueError, match="no gradient is recorded"):
                 call()
+
+
+# ------------------------------------------------------------------------- what large sizes do
+
+def test_the_large_sizes_of_norm_rope_reach_the_loops():
+    """of test_steps_large_gpu.py, from the number of workgroups that leave sums: a workgroup of 256 lanes has
+    256 / (lanes per head) groups, and a piece of its work is 4 heads a group and 16 tokens at most"""
+    import ctypes
+
+    import test_steps_large_gpu as large
+    import twg_capi as capi
+    P, L, sums = 1 << 20, capi.load(), {}
+    for name, (T, Hq, Hk, D, rot, axes, adjacent, dtype, longer) in large.ROPE.items():
+        d = capi.NormRope()
+        d.dtype, d.weight_dtype, d.position_dtype = capi.DTYPES[dtype], capi.DTYPES[torch.float32], capi.DTYPES[torch.int64]
+        d.norm, d.eps, d.n_axes, d.adjacent, d.head_dim, d.rot_dim = 1, 1e-6, axes, adjacent, D, rot
+        d.batch, d.tokens, d.positions, d.inv_freq = 1, T, P, P
+        for part, H in zip(d.part, (Hq, Hk)):
+            part.heads, part.x, part.dy, part.out, part.weight, part.dweight = H, P, P, P, P, P if H else None
+            part.x_stride[:] = T * H * (D + longer), H * (D + longer), D + longer
+            part.dy_stride[:] = part.out_stride[:] = T * H * D, H * D, D
+        workgroups = L.twg_norm_rope_backward_scratch_bytes(ctypes.byref(d)) // (4 * D)
+        size = 4 if dtype is torch.float32 else 2
+        lanes = max(1, D * size // 32)  # 2 runs of 16 bytes a lane
+        if longer:
+            lanes = D // 2  # one element a run
+        lanes = 1 << (lanes - 1).bit_length()
+        if "pieces" in name:
+            assert workgroups <= 4096
+            assert max(T / 16, T * (Hq + Hk) / (256 // lanes * 4)) > workgroups, name  # more than one piece each
+        else:
+            assert T * (Hq + Hk) > workgroups * (256 // lanes), name  # more than one head for a group
+        sums[name] = T * (Hq + Hk) * D * size * 2
+    for name, moved in sums.items():  # the forward call moves the least
+        assert ("hinted" in name) == (moved > 256 << 20 and large.ROPE[name][3:5] == (128, 128)), name
