@@ -292,3 +292,19 @@ def test_the_maximum_of_a_row_that_is_not_finite(rows, vocab, dtype):
         assert bool(torch.isnan(host(v)[:4]).all()) and not bool(torch.isnan(host(v)[4:]).any())
     grad = host(capi.token_logprobs_backward(dev(torch.ones(rows)), None, xd, td, got.row_max, got.row_sum))
     assert bool(torch.isnan(grad[:4]).all()) and not bool(torch.isnan(grad[4:]).any())
+
+
+# ------------------------------------------------------------------- where nothing flows back
+
+@pytest.mark.parametrize("how", ["F.dropout", "in place", "operator", "operator's residual", "twice"])
+def test_dropout_before_a_result_that_nothing_uses(how):
+    """the queries' heads come from a dropout, and only the keys' result is used"""
+    q, k = torch.randn(1, 3, 2, 16), torch.randn(1, 3, 1, 16)
+    qd, kd = dev(q, True), dev(k, True)
+    ops = torch.ops.webgpu
+    x = {"F.dropout": lambda: F.dropout(qd, 0.5), "in place": lambda: F.dropout(qd * 1.0, 0.5, inplace=True),
+         "operator": lambda: ops.dropout(qd, 0.5, 1), "operator's residual": lambda: ops.dropout(dev(q), 0.5, 1, 0, qd),
+         "twice": lambda: F.dropout(F.dropout(qd, 0.5), 0.5)}[how]()
+    yk = ops.norm_rope(x, kd, dev(torch.arange(3)), dev(torch.rand(8)))[1]
+    yk.backward(dev(torch.ones(1, 3, 1, 16)))
+    assert qd.grad is None and kd.grad is not None

@@ -471,6 +471,7 @@ struct Dropout : torch::autograd::Function<Dropout> {
     at::AutoDispatchBelowADInplaceOrView below;
     static const auto op = handle<decltype(dropout)>("webgpu::dropout");
     ctx->saved_data["p"] = p;
+    ctx->set_materialize_grads(false);  // (the device makes no zeros)
     ctx->saved_data["seed"] = seed;
     ctx->saved_data["offset"] = offset;
     ctx->saved_data["residual"] = residual.has_value() && residual->defined();
@@ -478,7 +479,7 @@ struct Dropout : torch::autograd::Function<Dropout> {
   }
   static variable_list backward(AutogradContext *ctx, variable_list grads) {
     at::Tensor gx;  // the mask is found again from the seed, the offset and the elements' places
-    if (ctx->needs_input_grad(0))
+    if (grads[0].defined() && ctx->needs_input_grad(0))
       gx = apply(grads[0], ctx->saved_data["p"].toDouble(), ctx->saved_data["seed"].toInt(),
                  ctx->saved_data["offset"].toInt(), MaybeTensor());
     const bool residual = ctx->saved_data["residual"].toBool() && ctx->needs_input_grad(1);
@@ -536,6 +537,7 @@ at::Tensor redo_dropout(const at::Tensor &x, double p, const at::Tensor &draw) {
 
 variable_list redone(AutogradContext *ctx, const variable_list &grads) {
   static const auto op = handle<decltype(redo_dropout)>("webgpu::_redo_dropout");
+  if (!grads[0].defined()) return {Variable(), Variable(), Variable()};  // nothing flows back
   return {op.call(grads[0], ctx->saved_data["p"].toDouble(), ctx->get_saved_variables()[0]), Variable(), Variable()};
 }
 
@@ -544,6 +546,7 @@ struct RedoDropout : torch::autograd::Function<RedoDropout> {
     at::AutoDispatchBelowADInplaceOrView below;
     static const auto op = handle<decltype(redo_dropout)>("webgpu::_redo_dropout");
     ctx->saved_data["p"] = p;
+    ctx->set_materialize_grads(false);  // (the device makes no zeros)
     ctx->save_for_backward({draw});
     return op.call(x, p, draw);
   }
@@ -559,6 +562,7 @@ struct DrawDropout : torch::autograd::Function<DrawDropout> {
     static const auto op = handle<decltype(draw_dropout)>("webgpu::_draw_dropout");
     const auto [out, draw] = op.call(x, p);
     ctx->saved_data["p"] = p;
+    ctx->set_materialize_grads(false);  // (the device makes no zeros)
     ctx->save_for_backward({draw});
     return out;
   }
@@ -575,6 +579,7 @@ struct DrawDropoutInPlace : torch::autograd::Function<DrawDropoutInPlace> {
     at::AutoDispatchBelowADInplaceOrView below;
     static const auto op = handle<decltype(draw_dropout_)>("webgpu::_draw_dropout_");
     ctx->saved_data["p"] = p;
+    ctx->set_materialize_grads(false);  // (the device makes no zeros)
     ctx->save_for_backward({op.call(x, p)});
     x.unsafeGetTensorImpl()->bump_version();
     ctx->mark_dirty({x});
