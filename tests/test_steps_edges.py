@@ -196,3 +196,12 @@ def test_the_large_sizes_of_norm_rope_reach_the_loops():
         sums[name] = T * (Hq + Hk) * D * size * 2
     for name, moved in sums.items():  # the forward call moves the least
         assert ("hinted" in name) == (moved > 256 << 20 and large.ROPE[name][3:5] == (128, 128)), name
+
+
+def test_norm_rope_backward_wants_a_gradient_for_each_input():
+    import twg_capi as capi
+    with FakeTensorMode():
+        q, k, f, pos = fake(1, 2, 3, 8), fake(1, 2, 1, 8), fake(4), torch.arange(2, device="webgpu")
+        for dq, dk, with_k in ((None, k, k), (q, None, k), (q, k, None), (q[:, :1], k, k), (q, k.to(torch.float16), k)):
+            with pytest.raises(ValueError):
+                capi.norm_rope_backward(dq, dk, q, with_k, pos, f)

@@ -502,7 +502,7 @@ def norm_rope_backward(dq, dk, q, k, positions, inv_freq, q_weight=None, k_weigh
             args += _NO_PART
             continue
         _same_device(x, dy)
-        if dy.shape != x.shape or dy.dtype != x.dtype:
+        if dy is None or dy.shape != x.shape or dy.dtype != x.dtype:
             raise ValueError("an incoming gradient must have its input's shape and dtype")
         x, dy = _dense_heads(x), _dense_heads(dy)
         keep.append((x, dy))
