@@ -308,3 +308,22 @@ def test_dropout_before_a_result_that_nothing_uses(how):
     yk = ops.norm_rope(x, kd, dev(torch.arange(3)), dev(torch.rand(8)))[1]
     yk.backward(dev(torch.ones(1, 3, 1, 16)))
     assert qd.grad is None and kd.grad is not None
+
+
+def test_dropout_in_place_on_tensors_of_inference_mode():
+    x = torch.randn(10)
+    torch.manual_seed(3)
+    with torch.inference_mode():
+        inside = dev(x)
+        F.dropout(inside, 0.5, inplace=True)
+        ref.assert_within(host(inside), *ref.dropout(x, 0.5, 3, 0))
+    normal = dev(x)
+    version = normal._version
+    with torch.inference_mode():
+        F.dropout(normal, 0.5, inplace=True)
+    assert normal._version > version
+    state = torch.webgpu.get_rng_state()
+    before = host(inside)
+    with pytest.raises(RuntimeError, match="[Ii]nference"):
+        F.dropout(inside, 0.5, inplace=True)
+    assert torch.equal(host(inside), before) and torch.equal(torch.webgpu.get_rng_state(), state)

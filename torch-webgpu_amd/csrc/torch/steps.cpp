@@ -604,6 +604,7 @@ at::Tensor aten_dropout_autograd(const at::Tensor &x, double p, bool train) {
 at::Tensor &aten_dropout_(at::Tensor &x, double p, bool train) {
   check_p(p);
   if (!train || p == 0 || x.numel() == 0) return x;
+  x.unsafeGetTensorImpl()->bump_version();  // (refuses a tensor of inference mode outside of it)
   draw_dropout_(x, p);
   return x;
 }
@@ -617,8 +618,8 @@ at::Tensor &aten_dropout_autograd_(at::Tensor &x, double p, bool train) {
   } else {
     at::AutoDispatchBelowADInplaceOrView below;
     static const auto op = handle<decltype(draw_dropout_)>("webgpu::_draw_dropout_");
-    op.call(x, p);
     x.unsafeGetTensorImpl()->bump_version();
+    op.call(x, p);
   }
   return x;
 }
