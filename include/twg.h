@@ -362,7 +362,7 @@ int twg_and(void *out, const void *a, const void *b, int32_t elem_size, const tw
  *  - Element types are TWG_DT_F16, TWG_DT_BF16 and TWG_DT_F32; arithmetic is binary32
  *    throughout and a result is rounded once, when it is stored.
  *  - The calls allocate nothing, never wait and keep nothing between calls, so they may be
- *    captured into a graph; where a call needs scratch, the caller brings it, and two calls
+ *    captured into a graph (after twg_init, which the first call would do); where a call needs scratch, the caller brings it, and two calls
  *    that may run at the same time need two.
  *  - TWG_STREAM_NULL names device 0's default (null) stream, which an opaque NULL
  *    cannot (NULL is the library's own stream).

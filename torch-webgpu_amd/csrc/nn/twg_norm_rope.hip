@@ -8,8 +8,8 @@
 // are the same for all of its heads: a workgroup computes them once for its tokens and keeps
 // cosines and sines in LDS.
 //
-// Bound by memory: 16384 tokens x 40 heads of 128 in bfloat16 (336 MB in and out) take 65 us forward and, with 503 MB,
-// 104 us backward (and 6 us for the weights' sums): 5.2 and 4.8 TB/s of the 6.7 that a large copy
+// Bound by memory: 16384 tokens x 40 heads of 128 in bfloat16 (336 MB in and out) take 64 us forward and, with 503 MB,
+// 101 us backward (and 6 us for the weights' sums): 5.3 and 5.0 TB/s of the 6.7 that a large copy
 // reaches.  The vector units are busy for half of that time (rotation, widening and rounding of 16 elements a
 // lane), which 4 wavefronts per SIMD do not hide entirely.  Calls below 20 us are bound by the chain
 // position -> angle -> barrier -> head and by the launch.
@@ -301,8 +301,9 @@ __global__ void __launch_bounds__(kThreads) rope_forward(RopeArgs a) {
 
 // The same walk, over as many pieces as there are for the workgroup, the group's next head on its way
 // while it works on one: its sums of dz u for the weight's gradient stay in registers until the last
-// piece is done.  Held to 128 registers (4 wavefronts per SIMD; it would take 132 and 3): 118 -> 108 us
-// for 16384 tokens x 40 heads of 128.
+// piece is done.  Held to 128 registers, 4 wavefronts per SIMD: heads of 16-bit elements in runs of 8 would take 132
+// (adjacent pairs 143), and 3.  They put 8 (12) bytes a lane into scratch for it.  16384 tokens x 40 heads of
+// 128 115 -> 106 us, adjacent 124 -> 117, x 24 heads of 64 51 -> 44; 4096 tokens x 40 39 -> 40.
 template <typename T, typename TW, int V, int C, bool ADJ, bool STREAM>
 __global__ void __launch_bounds__(kThreads, 4) rope_backward(RopeArgs a) {
   __shared__ TokenRoom room;
@@ -403,7 +404,8 @@ __global__ void __launch_bounds__(kThreads, 4) rope_backward(RopeArgs a) {
 }
 
 // Sum of the workgroups' partial rows, one part per grid row: 32 columns per workgroup, 32 lanes
-// down each column with eight rows on their way at a time.
+// down each column with eight rows on their way at a time.  Binary32 for a lane's rows (eight chains of at most 16),
+// binary64 for the 32 lanes' sums.
 struct SumArgs {
   const float *partial[2];
   int32_t rows[2];

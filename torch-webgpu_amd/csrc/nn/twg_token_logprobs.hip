@@ -315,7 +315,8 @@ __global__ void __launch_bounds__(64 * WAVES) logprobs_rows(LogprobArgs a) {
       b = nb;
     }
     // An entry of -inf makes the product 0 * -inf: from the first one on the wavefront keeps
-    // its exponents finite, one instruction more for each element.
+    // its exponents finite, one instruction more for each element.  A lane without an element counts as one: at
+    // a ragged end, and for the first wavefront of a row that does not begin on a pack's boundary.
     const Run before = r;
     if (!masked) {
 #pragma unroll
@@ -378,9 +379,10 @@ __global__ void __launch_bounds__(64 * WAVES) logprobs_rows(LogprobArgs a) {
   };
   // kUnroll packs of this lane, the first one pack `p` + threadIdx.x
   // The next step's packs are on their way while a lane looks at one step's (517 rows of 131072 float32
-  // with 5 alternatives 67 -> 53 us, 4096 rows of 8192 bfloat16 without 18.6 -> 15.3).  16-bit
-  // elements and alternatives together take too many registers for it (the same with 5 alternatives
-  // 29 -> 33 us).
+  // with 5 alternatives 67 -> 53 us, 4096 rows of 8192 bfloat16 without 18.6 -> 15.3).  With 16-bit
+  // elements and alternatives together it takes 102 registers instead of 87, and 4 wavefronts per SIMD are left of
+  // 5: 1100 rows of 50257 with 20 alternatives 39 -> 45 us, 4096 rows 109 -> 114; only 517 rows, whose
+  // workgroups leave room anyway, gain (28.9 -> 27.9).
   constexpr bool AHEAD = sizeof(T) == 4 || !TOP;
   Pack<T, E> coming[kUnroll];
   auto fetch = [&](int p, auto whole) {
@@ -681,9 +683,13 @@ struct RowShape {
   int splits;  // workgroups per row
 };
 
-// A row that one wavefront reads in two steps is one wavefront's.  Of longer rows, 1024 and more have
-// enough work in workgroups of 4 wavefronts; fewer take 8, and fewer than 256 are split into
-// workgroups of 4 that read one step of their own at least, about 1024 in all.
+// A row that one wavefront reads in two steps is one wavefront's.  Of longer rows, up to 512 are
+// workgroups of 8 wavefronts: with alternatives (87 registers) the chip holds 2 of those per compute unit, 512
+// in all, and one row more would wait for a second generation.  More rows take workgroups of 4, of which
+// 5 fit.  16-bit elements, 20 alternatives, 8 and 4 wavefronts: 512 rows of 50257 24 and 28 us, 517 rows
+// 35 and 29, 1023 rows 44 and 35; of 131072 38 and 45, 56 and 48, 70 and 57.  Without alternatives the two differ
+// by 10% either way there, float32 is alike.  Fewer than 256 rows are split into workgroups of 4 wavefronts
+// that read one step of their own at least, about 1024 in all.
 RowShape shape_of(const twg_token_logprobs_t *d) {
   const int64_t step = 16 * kUnroll / nn_size(d->dtype) * 64;  // elements a wavefront takes at a time
   if (d->vocab <= 2 * step) return RowShape{1, 1};

@@ -448,7 +448,7 @@ def norm_rope(q, k, positions, inv_freq, q_weight=None, k_weight=None, eps=1e-6,
     a head are rotated, the rest passes through); pair_axis: for each pair the position axis it
     follows (bytes or a list).  adjacent: pairs are neighbours (2i, 2i + 1) instead of halves.
     q_out / k_out: where the results go (unit stride along head_dim); q and k themselves for a
-    call in place."""
+    call in place, and no other memory that the call reads or writes."""
     stream = _stream_for(q)
     if torch.is_grad_enabled() and (  # (written out: a loop over the tensors takes longer)
             q.requires_grad or inv_freq.requires_grad or positions.requires_grad or (k is not None and k.requires_grad)
@@ -568,7 +568,7 @@ def token_logprobs_backward(g_logprob, g_entropy, logits, targets, row_max, row_
                             ignore_index=-100, out=None):
     """Gradient of the logits for the incoming gradients of logprob and entropy (either may be
     None).  row_max, row_sum and entropy come from token_logprobs with the same scale.  out may
-    be logits itself."""
+    be logits itself, and overlaps nothing else."""
     stream = _stream_for(logits)
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (g_logprob, g_entropy, out)):
         _refuse_unrecorded()
@@ -594,8 +594,9 @@ def token_logprobs_backward(g_logprob, g_entropy, logits, targets, row_max, row_
 def dropout(x, p, seed, offset=0, residual=None, out=None, d_offset=None):
     """residual + dropout(x), or dropout(x): elements are kept by Philox4x32-10 of (seed, offset,
     element index), so the gradient of x is dropout(grad, p, seed, offset) and no mask exists.  Each call of a
-    training step takes an offset of its own.  p is rounded to a multiple of 2^-16.  d_offset: an
-    int64 tensor of one element, added to offset when the kernel runs (captured graphs)."""
+    training step takes an offset of its own.  p is rounded to a multiple of 2^-16 (below
+    2^-17 nothing is dropped, above 1 - 2^-17 everything).  out may be x or residual itself, and overlaps
+    nothing else.  d_offset: an int64 tensor of one element, added to offset when the kernel runs (captured graphs)."""
     stream = _stream_for(x)
     if x.dtype not in _FLOATS:
         raise ValueError("x must be float16, bfloat16 or float32")
