@@ -13,8 +13,8 @@
 // Long rows are bound by memory and by vector instructions at nearly the same time: an element costs 5.5
 // (widen, maximum, multiply-add, exponential, sum, weighted sum), so that 2-byte elements at 6 TB/s keep
 // the vector units busy for three quarters of the time.  4096 x 131072: bfloat16 with 5
-// alternatives 177 us (6.1 TB/s), float32 327 us (6.6 TB/s).  Rows of a few thousand elements are
-// bound by the chain of a row's own steps: first maxima, lists, join.  The backward pass takes 184 us for
+// alternatives 176 us (6.1 TB/s), float32 314 us (6.8 TB/s).  Rows of a few thousand elements are
+// bound by the chain of a row's own steps: first maxima, lists, join.  The backward pass takes 183 us for
 // 2048 x 151643 bfloat16, a quarter of the rows without a gradient (5.9 TB/s).
 #include "twg_nn.h"
 
@@ -687,9 +687,10 @@ struct RowShape {
 // workgroups of 8 wavefronts: with alternatives (87 registers) the chip holds 2 of those per compute unit, 512
 // in all, and one row more would wait for a second generation.  More rows take workgroups of 4, of which
 // 5 fit.  16-bit elements, 20 alternatives, 8 and 4 wavefronts: 512 rows of 50257 24 and 28 us, 517 rows
-// 35 and 29, 1023 rows 44 and 35; of 131072 38 and 45, 56 and 48, 70 and 57.  Without alternatives the two differ
-// by 10% either way there, float32 is alike.  Fewer than 256 rows are split into workgroups of 4 wavefronts
-// that read one step of their own at least, about 1024 in all.
+// 35 and 29, 1023 rows 44 and 35; of 131072 38 and 45, 56 and 48, 70 and 57.  float32: 512 rows of 50257 28 and
+// 32, 517 rows 32 and 32.  Without alternatives, 256 rows of 131072 16 and 23, 512 rows 26 and 27, 512 rows of
+// 50257 16 and 15, 517 rows 20 and 17.  Fewer than 256 rows are split into workgroups of 4 wavefronts that
+// read one step of their own at least, about 1024 in all.
 RowShape shape_of(const twg_token_logprobs_t *d) {
   const int64_t step = 16 * kUnroll / nn_size(d->dtype) * 64;  // elements a wavefront takes at a time
   if (d->vocab <= 2 * step) return RowShape{1, 1};
