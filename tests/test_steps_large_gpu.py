@@ -161,3 +161,17 @@ def test_dropout_beyond_the_caches_share(dtype, residual, pitch):
     if not residual:  # binomial: 6 standard deviations, and p's rounding; an element of 0 counts as dropped
         kept = float((out != 0).double().mean()) + float((x == 0).double().mean())
         assert abs(kept - (1 - p)) < 6 * math.sqrt(p * (1 - p) / n) + 2.0 ** -15
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_dropout_of_more_than_2_to_the_32_elements(dtype):
+    n, p, seed = (1 << 32) + 4101, 0.5, 17
+    if torch.cuda.mem_get_info()[0] < 60 << 30:
+        pytest.skip("needs 60 GiB of GPU memory")
+    x = torch.ones(n, dtype=dtype, device="cuda")
+    capi.dropout(x, p, seed, out=x)
+    for first in (0, (1 << 31) - 100, (1 << 32) - 2000, n - 4000):
+        keep = ref.keep_mask(4000, p, seed, 0, first)
+        assert torch.equal(x[first:first + 4000].cpu() != 0, keep)
+    del x
+    torch.cuda.empty_cache()
